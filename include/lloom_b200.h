@@ -214,6 +214,27 @@ int lloom_b200_qmatmul_fwd_group(int w_dtype, int n_mats, const void *const *w_b
                                  const int64_t *ns, const int64_t *ldys, const int *stores, int64_t m, int64_t k,
                                  void *workspace, int64_t workspace_bytes, void *stream);
 
+/* ---- RMS norm in front of a product ----
+ * h = x + residual, rounded to x_type;  y = h / sqrt(mean(h^2) + eps) * weight, row by row.  residual NULL: h = x and
+ * `h` is not written.  y_type: x_type, or LLOOM_Q8_0 / LLOOM_Q8_K (lloom_b200_act_dtype of the weights that will read it): canonical
+ * activation blocks [m][k / block], those of lloom_b200_quantize_act on the f32 values of y.  The mean and 1 / sqrt are
+ * computed in 64 bits and rounded once, then h * (1 / sqrt) and the product with the weight are rounded to f32 each.
+ * x, residual: [m] rows of k elements of x_type, ldx / ldr elements apart; weight: k elements of w_type; h, y: contiguous.
+ * `h` may be the residual's own buffer where ldr == k; nothing else may overlap.  Types: LLOOM_F32, LLOOM_F16, LLOOM_BF16.
+ * Pointers are aligned to their elements, blocks to 4 bytes; rows and weights on 16 bytes with k a multiple of 8 are read faster. */
+int lloom_b200_rms_norm(const void *x, const void *residual, const void *weight, int x_type, int w_type, double eps, int64_t m, int64_t k,
+                        int64_t ldx, int64_t ldr, void *h, void *y, int y_type, void *stream);
+/* Activation blocks (LLOOM_Q8_0 / LLOOM_Q8_K) to the f32 values they stand for: scale * code.  out: 16-byte aligned. */
+int lloom_b200_dequantize_act(int act_dtype, const void *act_blocks, int64_t elem_count, float *out, void *stream);
+/* lloom_b200_qmatmul_fwd_typed and lloom_b200_qmatmul_fwd_group from canonical activation blocks [m][k / block], for any
+ * m and for m <= 8: no quantizer runs.  The kernels, and so the bits, are those of the forwards on values that quantize to these
+ * blocks.  Workspaces as there; w_image may be NULL; act_blocks 4-byte aligned. */
+int lloom_b200_qmatmul_fwd_acts(int w_dtype, const void *w_blocks, const void *w_image, const void *act_blocks, void *y, int y_type,
+                                int64_t m, int64_t n, int64_t k, int64_t ldy, void *workspace, int64_t workspace_bytes, void *stream);
+int lloom_b200_qmatmul_fwd_acts_group(int w_dtype, int n_mats, const void *const *w_blocks, const void *act_blocks, float *const *ys,
+                                      const int64_t *ns, const int64_t *ldys, const int *stores, int64_t m, int64_t k,
+                                      void *workspace, int64_t workspace_bytes, void *stream);
+
 /* ---- Routed mixture-of-experts forward: QCudaStorage::indexed_moe_forward (cuda.rs:505-622) ----
  * w_experts: [n_experts][n][k / block] canonical blocks (one stacked tensor, 16-byte aligned); x f32 [batch][in_dim1][k] with in_dim1 == 1 or topk; ids u32 [batch][topk] ON THE DEVICE;
  * out f32 [batch][topk][n]:  out[b][t] = W[ids[b][t]] . x[b][in_dim1 == 1 ? 0 : t].

@@ -54,6 +54,11 @@ SYMBOLS = [
     ("lloom_b200_peer_close", _int, [_vp]),
     ("lloom_b200_dequantize", _int, [_int, _vp, _i64, _vp, _int, _vp]),
     ("lloom_b200_get_rows", _int, [_int, _vp, _i64, _i64, _vp, _i64, _vp, _vp]),
+    ("lloom_b200_rms_norm", _int, [_vp, _vp, _vp, _int, _int, C.c_double, _i64, _i64, _i64, _i64, _vp, _vp, _int, _vp]),
+    ("lloom_b200_dequantize_act", _int, [_int, _vp, _i64, _vp, _vp]),
+    ("lloom_b200_qmatmul_fwd_acts", _int, [_int, _vp, _vp, _vp, _vp, _int, _i64, _i64, _i64, _i64, _vp, _i64, _vp]),
+    ("lloom_b200_qmatmul_fwd_acts_group", _int, [_int, _int, C.POINTER(_vp), _vp, C.POINTER(_vp), C.POINTER(_i64),
+                                                 C.POINTER(_i64), C.POINTER(_int), _i64, _i64, _vp, _i64, _vp]),
     # include/lloom_b200_host.h: C view of the C++ host layer
     ("lloom_b200_host_last_error", C.c_char_p, []),
     ("lloom_b200_host_quantize_rows", _int, [_int, _vp, _vp, _i64, _i64, _int]),

@@ -23,8 +23,12 @@ struct FwdIo {
 // lloom_b200_qmatmul_fwd (w_image == nullptr, store == LLOOM_STORE_PLAIN), _image and _store in one.
 int qmatmul_forward(int w_dtype, const void *w_blocks, const void *w_image, const void *x, void *y, int64_t m, int64_t n, int64_t k,
                     int64_t ldy, int store, void *workspace, int64_t workspace_bytes, void *stream, const FwdIo &io);
-int qmatmul_forward_group(int w_dtype, int n_mats, const void *const *w_blocks, const void *x, float *const *ys, const int64_t *ns,
-                          const int64_t *ldys, const int *stores, int64_t m, int64_t k, void *workspace, int64_t workspace_bytes,
+// The same from canonical activation blocks (lloom_b200_qmatmul_fwd_acts); io.x_type does not count
+int qmatmul_forward_acts(int w_dtype, const void *w_blocks, const void *w_image, const void *act, void *y, int64_t m, int64_t n, int64_t k,
+                         int64_t ldy, void *workspace, int64_t workspace_bytes, void *stream, const FwdIo &io);
+// Exactly one of act (canonical activation blocks) and x is non-null
+int qmatmul_forward_group(int w_dtype, int n_mats, const void *const *w_blocks, const void *act, const void *x, float *const *ys,
+                          const int64_t *ns, const int64_t *ldys, const int *stores, int64_t m, int64_t k, void *workspace, int64_t workspace_bytes,
                           void *stream, const FwdIo &io);
 // ids: 32-bit, or 64-bit of which the low half counts
 int indexed_moe_forward(int w_dtype, const void *w_experts, int64_t n_experts, int64_t n, int64_t k, const float *x, int64_t batch,
@@ -32,5 +36,9 @@ int indexed_moe_forward(int w_dtype, const void *w_experts, int64_t n_experts, i
                         int64_t workspace_bytes, void *stream, const FwdIo &io);
 int get_rows(int dtype, const void *blocks, int64_t rows, int64_t hidden, const void *ids, bool ids64, int64_t n_ids, float *out,
              void *stream, bool overlap);
+// lloom_b200_rms_norm, lloom_b200_dequantize_act (norm.cu)
+int rms_norm(const void *x, const void *residual, const void *weight, int x_type, int w_type, double eps, int64_t m, int64_t k, int64_t ldx,
+             int64_t ldr, void *h, void *y, int y_type, void *stream, bool overlap);
+int dequantize_act(int act_dtype, const void *act_blocks, int64_t elem_count, float *out, void *stream, bool overlap);
 
 }  // namespace lloom

@@ -1,6 +1,7 @@
 // C ABI of the library (see include/lloom_b200.h): argument checks, launch planning and dispatch.  The kernels live
 // in translation units of their own (gemv_*.cu, gemv_mma.cu, gemm.cu); this one holds the small ones (activation
 // quantizers, dequantize, the peer barrier).  No entry point on the forward path allocates, frees or synchronises.
+#include "abi.h"
 #include "common.cuh"
 #include "dequant.cuh"
 #include "forward.h"
@@ -40,7 +41,7 @@ void register_tu(const TuHooks &hooks) {
 
 static thread_local int t_last_cuda_error = 0;
 
-static int launch_status(cudaError_t e) {
+int launch_status(cudaError_t e) {
     if (e == cudaSuccess) return LLOOM_OK;
     t_last_cuda_error = (int)e;
     return LLOOM_ERR_LAUNCH;
@@ -53,21 +54,12 @@ static bool supported_weight(int dtype) {
     return false;
 }
 
-struct DeviceInfo {
-    int sm_count = 0;
-    int max_smem_optin = 0;   // per block
-    int smem_per_sm = 0;      // per multiprocessor
-    int smem_reserved = 0;    // per block, taken by the driver
-    int cc_major = 0;
-    bool ok = false;
-};
-
 // Launch overlap (programmatic dependent launch): lloom_b200_set_launch_overlap.
 static std::atomic<int> g_launch_overlap{-1};
 int launch_overlap() { return g_launch_overlap.load(std::memory_order_relaxed); }
 
 // Per-device attributes, queried once (the reference caches the same facts, fast_mmq.rs device-info cache).
-static int device_info(DeviceInfo &out) {
+int device_info(DeviceInfo &out) {
     static std::mutex mu;
     static DeviceInfo cache[64];
     int dev = 0;
@@ -294,7 +286,6 @@ static FwdIo default_io() {
     io.overlap = launch_overlap() > 0;
     return io;
 }
-static bool elem_type_ok(int t) { return t == LLOOM_F32 || t == LLOOM_F16 || t == LLOOM_BF16; }
 
 // What both decode kernels need to know of a launch.
 static void fill_params(GemvParams &p, int w_dtype, const void *w, const void *act, const void *x, void *y, int64_t m, int64_t n,
@@ -529,8 +520,6 @@ static int check_common(int w_dtype, int64_t m, int64_t n, int64_t k) {
     return LLOOM_OK;
 }
 
-static bool aligned(const void *p, uintptr_t a) { return ((uintptr_t)p & (a - 1)) == 0; }
-
 // ---- built-in scratch of lloom_b200_qmatmul_fwd_static ----
 // Lives in every device's copy of this module until the process exits.  In host code the name
 // below is only a host-side stand-in for the symbol, never a device address: the address a kernel
@@ -646,6 +635,21 @@ static int blocks_gemv(int w_dtype, const void *w_blocks, const void *act, void 
     return LLOOM_OK;
 }
 
+// The same from canonical blocks (m <= 8), by the kernels that decode_fwd takes.
+static int decode_acts(int w_dtype, const void *w_blocks, const void *act, void *y, int64_t m, int64_t n, int64_t k, int64_t ldy,
+                       void *scratch, void *stream, const FwdIo &io, const GemvOut *out) {
+    int rc;
+    if (m == 1 && !long_rows(w_dtype, k)) {
+        rc = gemv_launch(w_dtype, w_blocks, act, nullptr, y, m, n, k, ldy, (cudaStream_t)stream, io, out);
+        if (rc != LLOOM_ERR_SHAPE) return rc;
+    }
+    if (mma_fused(m, k)) {
+        rc = mma_launch(w_dtype, w_blocks, kActBlocks, act, y, m, n, k, ldy, (cudaStream_t)stream, io, out);
+        if (rc != LLOOM_ERR_SHAPE) return rc;
+    }
+    return mma_forward(w_dtype, w_blocks, act, nullptr, y, m, n, k, ldy, scratch, (cudaStream_t)stream, io, out);
+}
+
 // Prefill product (m > 8) after argument checks.  Activations: canonical blocks in `act`, or values in `x` (every kernel
 // quantizes them in the pass that lays them out).
 static int gemm_dispatch(int w_dtype, const void *w_blocks, const void *w_image, const void *act, const void *x,
@@ -685,12 +689,28 @@ int qmatmul_forward(int w_dtype, const void *w_blocks, const void *w_image, cons
     return gemm_dispatch(w_dtype, w_blocks, w_image, nullptr, x, y, m, n, k, ldy, workspace, stream, io);
 }
 
-int qmatmul_forward_group(int w_dtype, int n_mats, const void *const *w_blocks, const void *x, float *const *ys, const int64_t *ns,
-                          const int64_t *ldys, const int *stores, int64_t m, int64_t k, void *workspace, int64_t workspace_bytes,
+int qmatmul_forward_acts(int w_dtype, const void *w_blocks, const void *w_image, const void *act, void *y, int64_t m, int64_t n, int64_t k,
+                         int64_t ldy, void *workspace, int64_t workspace_bytes, void *stream, const FwdIo &io) {
+    int rc = check_common(w_dtype, m, n, k);
+    if (rc != LLOOM_OK) return rc;
+    if (ldy < n) return LLOOM_ERR_SHAPE;
+    if (!elem_type_ok(io.y_type)) return LLOOM_ERR_DTYPE;
+    if (!w_blocks || !act || !y) return LLOOM_ERR_NULL;
+    if (!workspace || workspace_bytes < product_scratch_bytes(w_dtype, m, n, k, w_image != nullptr)) return LLOOM_ERR_WORKSPACE;
+    if (!aligned(workspace, 256) || !aligned(w_blocks, 16) || !aligned(act, 4) || !aligned(y, 4) || !aligned(w_image, 1024))
+        return LLOOM_ERR_ALIGN;
+    if (m <= 8) return decode_acts(w_dtype, w_blocks, act, y, m, n, k, ldy, workspace, stream, io, nullptr);
+    if (w_image && lloom_b200_weight_image_bytes(w_dtype, n, k) <= 0) return LLOOM_ERR_SHAPE;
+    return gemm_dispatch(w_dtype, w_blocks, w_image, act, nullptr, y, m, n, k, ldy, workspace, stream, io);
+}
+
+int qmatmul_forward_group(int w_dtype, int n_mats, const void *const *w_blocks, const void *act, const void *x, float *const *ys,
+                          const int64_t *ns, const int64_t *ldys, const int *stores, int64_t m, int64_t k, void *workspace, int64_t workspace_bytes,
                           void *stream, const FwdIo &io) {
     if (!elem_type_ok(io.x_type) || io.y_type != LLOOM_F32) return LLOOM_ERR_DTYPE;
     if (n_mats < 1 || n_mats > kMaxGroup) return LLOOM_ERR_SHAPE;
-    if (!w_blocks || !x || !ys || !ns || !ldys) return LLOOM_ERR_NULL;
+    if (!w_blocks || (!act && !x) || !ys || !ns || !ldys) return LLOOM_ERR_NULL;
+    if (act && x) return LLOOM_ERR_SHAPE;
     if (m > 8) return LLOOM_ERR_SHAPE;
     GemvGroup group;
     group.count = n_mats;
@@ -714,7 +734,7 @@ int qmatmul_forward_group(int w_dtype, int n_mats, const void *const *w_blocks, 
     if (n_total > (1ll << 30)) return LLOOM_ERR_SHAPE;
     const int64_t need = lloom_b200_workspace_bytes(w_dtype, m, n_max, k);
     if (!workspace || workspace_bytes < need) return LLOOM_ERR_WORKSPACE;
-    if (!aligned(workspace, 256) || !aligned(x, 16)) return LLOOM_ERR_ALIGN;
+    if (!aligned(workspace, 256) || !aligned(x, 16) || !aligned(act, 4)) return LLOOM_ERR_ALIGN;
     int rc;
     // One launch of the dp4a kernel for the whole group: one row, where it is the decode path anyway, and two rows of up to
     // 40 MB, where it spares a quantizer and a launch per matrix (graph, Q4_K / Q8_0: q|k|v of a 4096-wide model 11.5 -> 7.9, 14.3 ->
@@ -722,21 +742,23 @@ int qmatmul_forward_group(int w_dtype, int n_mats, const void *const *w_blocks, 
     // 21.5 -> 21.2, 34.3 -> 31.4; Q4_0 26.4 -> 28.3) and lose in a layer, whose next launches cannot start beside them (Q4_K
     // layer with groups 49.3 -> 55.8, Q8_0 70.5 -> 73.0).
     if (n_mats > 1 && (m == 1 || (m == 2 && n_total * weight_row_bytes(w_dtype, k) <= (40 << 20)))) {
-        rc = gemv_launch(w_dtype, nullptr, nullptr, x, nullptr, m, 0, k, 0, (cudaStream_t)stream, io, nullptr, &group);
+        rc = gemv_launch(w_dtype, nullptr, act, x, nullptr, m, 0, k, 0, (cudaStream_t)stream, io, nullptr, &group);
         if (rc != LLOOM_ERR_SHAPE) return rc;
     }
     // Otherwise the activations are quantized once and every matrix gets its own launch.
     uint8_t *scratch = (uint8_t *)workspace;
     if (m > 1) {
         const MmaActs acts = mma_acts(w_dtype, m);
-        rc = launch_status(launch_quantize_image(w_dtype, x, io.x_type, scratch, m, k, acts.tiles, acts.group_nt, io.overlap,
-                                                 (cudaStream_t)stream));
+        rc = launch_status(act ? launch_blocks_image(w_dtype, act, scratch, m, k, acts.group_nt, (cudaStream_t)stream)
+                               : launch_quantize_image(w_dtype, x, io.x_type, scratch, m, k, acts.tiles, acts.group_nt, io.overlap,
+                                                       (cudaStream_t)stream));
         if (rc != LLOOM_OK) return rc;
     }
     for (int g = 0; g < n_mats; ++g) {
         GemvOut out;
         out.store = group.store[g];
         rc = m > 1 ? mma_launch(w_dtype, group.w[g], kActImage, scratch, group.y[g], m, group.n[g], k, group.ldy[g], (cudaStream_t)stream, io, &out)
+             : act ? decode_acts(w_dtype, group.w[g], act, group.y[g], m, group.n[g], k, group.ldy[g], scratch, stream, io, &out)
                    : decode_fwd(w_dtype, group.w[g], x, group.y[g], m, group.n[g], k, group.ldy[g], scratch, stream, io, &out);
         if (rc != LLOOM_OK) return rc;
     }
@@ -990,8 +1012,22 @@ int lloom_b200_qmatmul_fwd_store(int w_dtype, const void *w_blocks, const float 
 int lloom_b200_qmatmul_fwd_group(int w_dtype, int n_mats, const void *const *w_blocks, const float *x, float *const *ys,
                                  const int64_t *ns, const int64_t *ldys, const int *stores, int64_t m, int64_t k,
                                  void *workspace, int64_t workspace_bytes, void *stream) {
-    return qmatmul_forward_group(w_dtype, n_mats, w_blocks, x, ys, ns, ldys, stores, m, k, workspace, workspace_bytes, stream,
+    return qmatmul_forward_group(w_dtype, n_mats, w_blocks, nullptr, x, ys, ns, ldys, stores, m, k, workspace, workspace_bytes, stream,
                                  default_io());
+}
+
+int lloom_b200_qmatmul_fwd_acts(int w_dtype, const void *w_blocks, const void *w_image, const void *act_blocks, void *y, int y_type,
+                                int64_t m, int64_t n, int64_t k, int64_t ldy, void *workspace, int64_t workspace_bytes, void *stream) {
+    FwdIo io = default_io();
+    io.y_type = y_type;
+    return qmatmul_forward_acts(w_dtype, w_blocks, w_image, act_blocks, y, m, n, k, ldy, workspace, workspace_bytes, stream, io);
+}
+
+int lloom_b200_qmatmul_fwd_acts_group(int w_dtype, int n_mats, const void *const *w_blocks, const void *act_blocks, float *const *ys,
+                                      const int64_t *ns, const int64_t *ldys, const int *stores, int64_t m, int64_t k,
+                                      void *workspace, int64_t workspace_bytes, void *stream) {
+    return qmatmul_forward_group(w_dtype, n_mats, w_blocks, act_blocks, nullptr, ys, ns, ldys, stores, m, k, workspace, workspace_bytes,
+                                 stream, default_io());
 }
 
 int lloom_b200_indexed_moe_forward(int w_dtype, const void *w_experts, int64_t n_experts, int64_t n, int64_t k,

@@ -217,6 +217,49 @@ PyObject *Storage_forward(PyObject *o, PyObject *const *args, Py_ssize_t nargs) 
     END_HANDLE_TH_ERRORS
 }
 
+// Contiguous canonical activation blocks [.., row bytes] of this storage's device, for rows of k elements
+bool blocks_ok(const Storage *self, const at::Tensor &a, int64_t k) {
+    const int64_t row = lloom_b200_act_row_bytes(self->dtype, k);
+    return a.defined() && a.device() == self->data->device() && a.layout() == at::kStrided && a.scalar_type() == at::kByte && row > 0 &&
+           a.dim() >= 2 && a.size(-1) == row && a.numel() > 0 && a.is_contiguous();
+}
+
+at::ScalarType scalar_of(int type) { return type == LLOOM_F16 ? at::kHalf : type == LLOOM_BF16 ? at::kBFloat16 : at::kFloat; }
+
+// forward_acts(blocks, (n, k), element type of the result) -> [.., n]
+PyObject *Storage_forward_acts(PyObject *o, PyObject *const *args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    Storage *self = reinterpret_cast<Storage *>(o);
+    int64_t n, k;
+    if (nargs != 3 || !THPVariable_Check(args[0]) || !shape2(args[1], n, k)) return none_or_error();
+    const int y_type = (int)PyLong_AsLong(args[2]);
+    if (PyErr_Occurred()) return nullptr;
+    const at::Tensor &a = THPVariable_Unpack(args[0]);
+    if (!blocks_ok(self, a, k)) Py_RETURN_NONE;
+    const c10::Device dev = self->data->device();
+    c10::cuda::CUDAGuard guard(dev);
+    const int64_t m = a.numel() / a.size(-1);
+    const bool image = self->image && m > 8;
+    const int64_t need = image ? lloom_b200_workspace_bytes_with_image(self->dtype, m, n, k)
+                               : lloom_b200_workspace_bytes(self->dtype, m, n, k);
+    if (need <= 0) Py_RETURN_NONE;
+    c10::SmallVector<int64_t, 5> sizes(a.sizes().begin(), a.sizes().end());
+    sizes.back() = n;
+    at::Tensor y = at::detail::empty_cuda(sizes, scalar_of(y_type), dev, std::nullopt);
+    FwdIo io;
+    io.overlap = overlaps(self);
+    io.y_type = y_type;
+    const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
+    const at::Tensor &ws = workspaces().get(dev, stream, need);
+    const int rc = lloom::qmatmul_forward_acts(self->dtype, self->data->const_data_ptr(),
+                                               image ? static_cast<char *>(self->image->data_ptr()) + self->image_off : nullptr,
+                                               a.const_data_ptr(), y.data_ptr(), m, n, k, n, ws.data_ptr(), ws.numel(), stream, io);
+    if (rc != LLOOM_OK) return fail(rc, "qmatmul_fwd_acts");
+    self->settled = true;
+    return THPVariable_Wrap(y);
+    END_HANDLE_TH_ERRORS
+}
+
 // embedding(ids, (rows, hidden)) -> f32 ids.shape + [hidden]
 PyObject *Storage_embedding(PyObject *o, PyObject *const *args, Py_ssize_t nargs) {
     HANDLE_TH_ERRORS
@@ -277,10 +320,10 @@ PyObject *Storage_experts(PyObject *o, PyObject *const *args, Py_ssize_t nargs) 
 }
 
 
-// group(storages, (n, ..), k, x, stores or None, outs or None) -> list of f32 [.., n_g]
+// group(storages, (n, ..), k, x, stores or None, outs or None, whether x is activation blocks) -> list of f32 [.., n_g]
 PyObject *module_group(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
     HANDLE_TH_ERRORS
-    if (nargs != 6 || !PyList_Check(args[0]) || !PyList_Check(args[1]) || !THPVariable_Check(args[3])) Py_RETURN_NONE;
+    if (nargs != 7 || !PyList_Check(args[0]) || !PyList_Check(args[1]) || !THPVariable_Check(args[3])) Py_RETURN_NONE;
     const Py_ssize_t G = PyList_GET_SIZE(args[0]);
     if (G < 1 || G > LLOOM_B200_MAX_GROUP || PyList_GET_SIZE(args[1]) != G) Py_RETURN_NONE;
     const int64_t k = PyLong_AsLongLong(args[2]);
@@ -309,10 +352,11 @@ PyObject *module_group(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
         io.overlap = io.overlap && overlaps(st[g]);
     }
     int x_type;
-    if (!acts_ok(st[0], x, k, x_type) || x_type != LLOOM_F32) Py_RETURN_NONE;
+    const bool blocks = args[6] == Py_True;
+    if (blocks ? !blocks_ok(st[0], x, k) : !acts_ok(st[0], x, k, x_type) || x_type != LLOOM_F32) Py_RETURN_NONE;
     const c10::Device dev = st[0]->data->device();
     c10::cuda::CUDAGuard guard(dev);
-    const int64_t m = x.numel() / k;
+    const int64_t m = x.numel() / x.size(-1);
     const int64_t need = lloom_b200_workspace_bytes(st[0]->dtype, m, n_max, k);
     if (need <= 0) Py_RETURN_NONE;
     THPObjectPtr list(PyList_New(G));
@@ -339,11 +383,88 @@ PyObject *module_group(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
     }
     const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
     const at::Tensor &ws = workspaces().get(dev, stream, need);
-    const int rc = lloom::qmatmul_forward_group(st[0]->dtype, (int)G, w, x.const_data_ptr(), y, n, ld, store, m, k, ws.data_ptr(),
+    const int rc = lloom::qmatmul_forward_group(st[0]->dtype, (int)G, w, blocks ? x.const_data_ptr() : nullptr,
+                                                blocks ? nullptr : x.const_data_ptr(), y, n, ld, store, m, k, ws.data_ptr(),
                                                 ws.numel(), stream, io);
     if (rc != LLOOM_OK) return fail(rc, "qmatmul_fwd_group");
     for (Py_ssize_t g = 0; g < G; ++g) st[g]->settled = true;
     return list.release();
+    END_HANDLE_TH_ERRORS
+}
+
+// The rows of [.., k] and how far apart they are: a contiguous tensor, or a matrix whose rows are
+bool row_layout(const at::Tensor &t, int64_t &rows, int64_t &k, int64_t &ld) {
+    if (!t.defined() || t.layout() != at::kStrided || !t.is_cuda() || t.dim() < 1) return false;
+    k = t.size(-1);
+    if (k == 0) return false;
+    rows = t.numel() / k;
+    ld = k;
+    if (t.is_contiguous()) return true;
+    if (t.dim() != 2 || t.stride(1) != 1 || t.stride(0) < k) return false;
+    ld = t.stride(0);
+    return true;
+}
+
+// rms_norm(x, weight, eps, residual or None, -1 or the block type) -> y, or (y, h) with a residual
+PyObject *module_rms_norm(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    if (nargs != 5 || !THPVariable_Check(args[0]) || !THPVariable_Check(args[1]) || (args[3] != Py_None && !THPVariable_Check(args[3])))
+        Py_RETURN_NONE;
+    const at::Tensor &x = THPVariable_Unpack(args[0]), &w = THPVariable_Unpack(args[1]);
+    const double eps = PyFloat_AsDouble(args[2]);
+    const int blocks = (int)PyLong_AsLong(args[4]);
+    if (PyErr_Occurred()) return nullptr;
+    int64_t m, k, ldx, rm, rk, ldr = 0;
+    int x_type, w_type;
+    if (!row_layout(x, m, k, ldx) || !elem_type(x.scalar_type(), x_type)) Py_RETURN_NONE;
+    if (!w.defined() || w.device() != x.device() || w.dim() != 1 || w.size(0) != k || !w.is_contiguous() || !elem_type(w.scalar_type(), w_type))
+        Py_RETURN_NONE;
+    at::Tensor r;
+    if (args[3] != Py_None) {
+        r = THPVariable_Unpack(args[3]);
+        if (!row_layout(r, rm, rk, ldr) || r.scalar_type() != x.scalar_type() || r.device() != x.device() || r.sizes() != x.sizes()) Py_RETURN_NONE;
+    }
+    const int64_t be = blocks >= 0 ? lloom_b200_block_elems(blocks) : 1;
+    if (be <= 0 || k % be != 0) Py_RETURN_NONE;
+    const c10::Device dev = x.device();
+    c10::cuda::CUDAGuard guard(dev);
+    c10::SmallVector<int64_t, 5> sizes(x.sizes().begin(), x.sizes().end());
+    at::Tensor h, y;
+    if (r.defined()) h = at::detail::empty_cuda(sizes, x.scalar_type(), dev, std::nullopt);
+    if (blocks >= 0) sizes.back() = k / be * lloom_b200_block_bytes(blocks);
+    y = at::detail::empty_cuda(sizes, blocks >= 0 ? at::kByte : x.scalar_type(), dev, std::nullopt);
+    if (m > 0) {
+        const int rc = lloom::rms_norm(x.const_data_ptr(), r.defined() ? r.const_data_ptr() : nullptr, w.const_data_ptr(), x_type, w_type, eps,
+                                       m, k, ldx, ldr, r.defined() ? h.data_ptr() : nullptr, y.data_ptr(), blocks >= 0 ? blocks : x_type,
+                                       c10::cuda::getCurrentCUDAStream(dev.index()).stream(), lloom::launch_overlap() != 0);
+        if (rc != LLOOM_OK) return fail(rc, "rms_norm");
+    }
+    if (!r.defined()) return THPVariable_Wrap(y);
+    THPObjectPtr yo(THPVariable_Wrap(y)), ho(THPVariable_Wrap(h));
+    return yo && ho ? PyTuple_Pack(2, yo.get(), ho.get()) : nullptr;
+    END_HANDLE_TH_ERRORS
+}
+
+// dequantize_act(blocks [.., row bytes], block type) -> f32 [.., k]
+PyObject *module_dequantize_act(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    if (nargs != 2 || !THPVariable_Check(args[0])) Py_RETURN_NONE;
+    const at::Tensor &a = THPVariable_Unpack(args[0]);
+    const int type = (int)PyLong_AsLong(args[1]);
+    if (PyErr_Occurred()) return nullptr;
+    const int64_t be = lloom_b200_block_elems(type), bb = lloom_b200_block_bytes(type);
+    if (!a.defined() || !a.is_cuda() || a.scalar_type() != at::kByte || !a.is_contiguous() || a.dim() < 1 || be <= 0 || a.size(-1) % bb != 0)
+        Py_RETURN_NONE;
+    c10::cuda::CUDAGuard guard(a.device());
+    c10::SmallVector<int64_t, 5> sizes(a.sizes().begin(), a.sizes().end());
+    sizes.back() = sizes.back() / bb * be;
+    at::Tensor out = at::detail::empty_cuda(sizes, at::kFloat, a.device(), std::nullopt);
+    if (out.numel() > 0) {
+        const int rc = lloom::dequantize_act(type, a.const_data_ptr(), out.numel(), out.data_ptr<float>(),
+                                             c10::cuda::getCurrentCUDAStream(a.device().index()).stream(), lloom::launch_overlap() != 0);
+        if (rc != LLOOM_OK) return fail(rc, "dequantize_act");
+    }
+    return THPVariable_Wrap(out);
     END_HANDLE_TH_ERRORS
 }
 
@@ -369,6 +490,7 @@ PyObject *module_set_error(PyObject *, PyObject *fn) {
 
 #define FAST(fn) reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(fn))
 PyMethodDef storage_methods[] = {{"forward", FAST(Storage_forward), METH_FASTCALL, nullptr},
+                                 {"forward_acts", FAST(Storage_forward_acts), METH_FASTCALL, nullptr},
                                  {"embedding", FAST(Storage_embedding), METH_FASTCALL, nullptr},
                                  {"experts", FAST(Storage_experts), METH_FASTCALL, nullptr},
                                  {"set_image", Storage_set_image, METH_VARARGS, nullptr},
@@ -378,6 +500,8 @@ PyMethodDef storage_methods[] = {{"forward", FAST(Storage_forward), METH_FASTCAL
                                  {nullptr, nullptr, 0, nullptr}};
 
 PyMethodDef module_methods[] = {{"group", FAST(module_group), METH_FASTCALL, nullptr},
+                                {"rms_norm", FAST(module_rms_norm), METH_FASTCALL, nullptr},
+                                {"dequantize_act", FAST(module_dequantize_act), METH_FASTCALL, nullptr},
                                 {"workspace", module_workspace, METH_VARARGS, nullptr},
                                 {"set_error", module_set_error, METH_O, nullptr},
                                 {nullptr, nullptr, 0, nullptr}};

@@ -336,6 +336,53 @@ class QTensor:
         return out
 
 
+_ELEM_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}
+_ACT_TYPES = {GgmlDType.Q4_0: GgmlDType.Q8_0, GgmlDType.Q5_0: GgmlDType.Q8_0, GgmlDType.Q8_0: GgmlDType.Q8_0,
+              GgmlDType.Q4K: GgmlDType.Q8K, GgmlDType.Q5K: GgmlDType.Q8K, GgmlDType.Q6K: GgmlDType.Q8K}
+
+
+class QActs:
+    """Activations as the canonical blocks that the products read (``VecDotType``, k_quants.rs:717, 1507, 2082): ``blocks``
+    uint8 ``[.., row bytes]``, ``dtype`` Q8_0 or Q8K, ``shape`` ``[.., k]``.  Made by ``rms_norm(.., act_for=..)`` or, from
+    values, by ``quantize``."""
+
+    __slots__ = ("blocks", "dtype", "shape")
+
+    def __init__(self, blocks: torch.Tensor, dtype: GgmlDType):
+        dtype = GgmlDType(dtype)
+        if dtype not in (GgmlDType.Q8_0, GgmlDType.Q8K):
+            raise LloomError(_lib.ERR_DTYPE, "QActs", f"{dtype!r} is not an activation block type")
+        be, bb = _ACT_BLOCK[dtype]
+        if blocks.dtype != torch.uint8 or blocks.dim() < 1 or blocks.shape[-1] % bb != 0:
+            raise LloomError(_lib.ERR_SHAPE, "QActs", f"{tuple(blocks.shape)} {blocks.dtype} is not rows of {dtype!r} blocks")
+        self.blocks, self.dtype = blocks, dtype
+        self.shape = (*blocks.shape[:-1], blocks.shape[-1] // bb * be)
+
+    @classmethod
+    def quantize(cls, x: torch.Tensor, act_for: GgmlDType) -> "QActs":
+        """f32 ``[m, k]`` to the blocks that weights of type ``act_for`` are dotted with."""
+        return cls(quantize_act(GgmlDType(act_for), x), act_type(act_for))
+
+    def dequantize(self) -> torch.Tensor:
+        """The f32 values the blocks stand for."""
+        out = _native().dequantize_act(self.blocks, self.dtype)
+        if out is None:
+            raise LloomError(_lib.ERR_SHAPE, "QActs.dequantize", f"blocks {tuple(self.blocks.shape)} on {self.blocks.device}: "
+                                                                 "contiguous on the GPU is wanted")
+        return out
+
+
+_ACT_BLOCK = {GgmlDType.Q8_0: (32, 34), GgmlDType.Q8K: (256, 292)}
+
+
+def act_type(w_dtype: GgmlDType) -> GgmlDType:
+    """The activation block type that weights of this type are dotted with."""
+    t = _ACT_TYPES.get(w_dtype)
+    if t is None:
+        raise LloomError(_lib.ERR_DTYPE, "act_type", f"{w_dtype!r} is not a weight type of this backend")
+    return t
+
+
 class QMatMul:
     """``QMatMul::QTensor`` arm (mod.rs:1698-1752): ``forward(xs) = xs @ W^T`` over packed weights."""
 
@@ -354,6 +401,22 @@ class QMatMul:
         return y if y is not None else qt.fwd(xs)
 
     __call__ = forward
+
+    def forward_quantized(self, acts: QActs, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+        """``acts @ W^T`` for activations that are blocks already (``rms_norm(.., act_for=..)``): no quantizer runs, and the
+        result is that of ``forward`` on f32 values that quantize to these blocks, bit for bit.  ``dtype``: of the result."""
+        qt = self.qtensor
+        n, k = qt.shape
+        if acts.dtype != _ACT_TYPES[qt.dtype()] or acts.shape[-1] != k:
+            raise LloomError(_lib.ERR_SHAPE, "forward_quantized",
+                             f"{acts.dtype!r} activations {tuple(acts.shape)} do not fit {qt.dtype()!r} weights {(n, k)}")
+        if dtype not in _ELEM_TYPES:
+            raise LloomError(_lib.ERR_DTYPE, "forward_quantized", f"results are f32, f16 or bf16, not {dtype}")
+        y = qt.storage._native.forward_acts(acts.blocks, (n, k), _ELEM_TYPES[dtype])
+        if y is None:
+            raise LloomError(_lib.ERR_SHAPE, "forward_quantized",
+                             f"blocks {tuple(acts.blocks.shape)} on {acts.blocks.device} for weights {(n, k)} on {qt.device()}")
+        return y
 
     MV_STORE_MAX_ROWS = 8
 
@@ -386,19 +449,21 @@ class QMatMul:
         return gate
 
 
-def forward_group(mats: Sequence["QMatMul"], xs: torch.Tensor, stores: Sequence[int] | None = None,
+def forward_group(mats: Sequence["QMatMul"], xs: "torch.Tensor | QActs", stores: Sequence[int] | None = None,
                   outs: Sequence[torch.Tensor] | None = None) -> list[torch.Tensor]:
     """Decode forward of several ``QMatMul`` that share the input ``xs`` (gate|up, q|k|v) through
     ``lloom_b200_qmatmul_fwd_group``: one activation read and, for a single row, one launch for all of them.
     All weights must have the same dtype, k and device; at most 8 rows.  ``stores[g]``: block on matrix g's store
-    (0 plain, 1 SiLU, 2 multiply into ``outs[g]``).  Each result equals that matrix's own ``forward`` bit for bit."""
+    (0 plain, 1 SiLU, 2 multiply into ``outs[g]``).  Each result equals that matrix's own ``forward`` bit for bit.
+    ``xs`` may be activation blocks (``QActs``): each result then equals ``forward_quantized``."""
     if not 1 <= len(mats) <= 8:
         raise LloomError(_lib.ERR_SHAPE, "forward_group", "1 to 8 matrices")
     tensors = [mm.qtensor for mm in mats]
     k = tensors[0].shape[1]
-    if all(t.shape[1] == k for t in tensors):
-        got = _native().group([t.storage._native for t in tensors], [t.shape[0] for t in tensors], k, xs,
-                              None if stores is None else list(stores), None if outs is None else list(outs))
+    blocks = isinstance(xs, QActs)
+    if all(t.shape[1] == k for t in tensors) and not (blocks and xs.dtype != _ACT_TYPES[tensors[0].dtype()]):
+        got = _native().group([t.storage._native for t in tensors], [t.shape[0] for t in tensors], k, xs.blocks if blocks else xs,
+                              None if stores is None else list(stores), None if outs is None else list(outs), blocks)
         if got is not None:
             return got
     dt, dev = tensors[0].dtype(), tensors[0].device()

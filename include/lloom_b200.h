@@ -235,6 +235,26 @@ int lloom_b200_qmatmul_fwd_acts_group(int w_dtype, int n_mats, const void *const
                                       const int64_t *ns, const int64_t *ldys, const int *stores, int64_t m, int64_t k,
                                       void *workspace, int64_t workspace_bytes, void *stream);
 
+/* ---- Microscaled 4-bit floating point (OCP MX: E2M1 elements, an E8M0 scale per 32 elements of a row) ----
+ * Weights are kept as the image that the tensor cores read (4.25 bits an element; rows padded to 128, k to 256): one device
+ * buffer, 256-byte aligned, written by lloom_b200_mx_quantize (from f32 / f16 / bf16 values [rows][k]) or
+ * lloom_b200_mx_from_blocks (from a file's MXFP4 blocks on the device, ggml type 39: 17 bytes per 32 elements, E8M0 scale, then elements 0..15
+ * in the low and 16..31 in the high halves of 16 bytes), and read back by the other two.  k is a multiple of 32.
+ *   quantisation: scale 2^e, e = floor(log2 max|v|) - 2 within [-127, 127]; codes to nearest, ties to even, beyond 6 to 6; a block that
+ *   holds a NaN or an infinity gets the scale NaN.
+ * lloom_b200_mx_fwd: y[m][n] = x . W^T with x quantized to the same format on the way; products of codes are exact, sums are f32.
+ * x [m][k] contiguous, 16-byte aligned; y [m][ldy]; any m.  Types LLOOM_F32, LLOOM_F16, LLOOM_BF16.  workspace:
+ * lloom_b200_mx_workspace_bytes, 256-byte aligned.  0 bytes = refused shape. */
+#define LLOOM_MXFP4 39
+int64_t lloom_b200_mx_image_bytes(int64_t rows, int64_t k);
+int lloom_b200_mx_quantize(const void *x, int x_type, int64_t rows, int64_t k, void *image, int64_t image_bytes, void *stream);
+int lloom_b200_mx_from_blocks(const void *blocks, int64_t rows, int64_t k, void *image, int64_t image_bytes, void *stream);
+int lloom_b200_mx_to_blocks(const void *image, int64_t rows, int64_t k, void *blocks, void *stream);
+int lloom_b200_mx_dequantize(const void *image, int64_t rows, int64_t k, void *out, int out_is_f16, void *stream);
+int64_t lloom_b200_mx_workspace_bytes(int64_t m, int64_t n, int64_t k);
+int lloom_b200_mx_fwd(const void *image, const void *x, int x_type, void *y, int y_type, int64_t m, int64_t n, int64_t k, int64_t ldy,
+                      void *workspace, int64_t workspace_bytes, void *stream);
+
 /* ---- Routed mixture-of-experts forward: QCudaStorage::indexed_moe_forward (cuda.rs:505-622) ----
  * w_experts: [n_experts][n][k / block] canonical blocks (one stacked tensor, 16-byte aligned); x f32 [batch][in_dim1][k] with in_dim1 == 1 or topk; ids u32 [batch][topk] ON THE DEVICE;
  * out f32 [batch][topk][n]:  out[b][t] = W[ids[b][t]] . x[b][in_dim1 == 1 ? 0 : t].

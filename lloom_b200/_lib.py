@@ -59,6 +59,13 @@ SYMBOLS = [
     ("lloom_b200_qmatmul_fwd_acts", _int, [_int, _vp, _vp, _vp, _vp, _int, _i64, _i64, _i64, _i64, _vp, _i64, _vp]),
     ("lloom_b200_qmatmul_fwd_acts_group", _int, [_int, _int, C.POINTER(_vp), _vp, C.POINTER(_vp), C.POINTER(_i64),
                                                  C.POINTER(_i64), C.POINTER(_int), _i64, _i64, _vp, _i64, _vp]),
+    ("lloom_b200_mx_image_bytes", _i64, [_i64, _i64]),
+    ("lloom_b200_mx_quantize", _int, [_vp, _int, _i64, _i64, _vp, _i64, _vp]),
+    ("lloom_b200_mx_from_blocks", _int, [_vp, _i64, _i64, _vp, _i64, _vp]),
+    ("lloom_b200_mx_to_blocks", _int, [_vp, _i64, _i64, _vp, _vp]),
+    ("lloom_b200_mx_dequantize", _int, [_vp, _i64, _i64, _vp, _int, _vp]),
+    ("lloom_b200_mx_workspace_bytes", _i64, [_i64, _i64, _i64]),
+    ("lloom_b200_mx_fwd", _int, [_vp, _vp, _int, _vp, _int, _i64, _i64, _i64, _i64, _vp, _i64, _vp]),
     # include/lloom_b200_host.h: C view of the C++ host layer
     ("lloom_b200_host_last_error", C.c_char_p, []),
     ("lloom_b200_host_quantize_rows", _int, [_int, _vp, _vp, _i64, _i64, _int]),

@@ -40,5 +40,10 @@ int get_rows(int dtype, const void *blocks, int64_t rows, int64_t hidden, const 
 int rms_norm(const void *x, const void *residual, const void *weight, int x_type, int w_type, double eps, int64_t m, int64_t k, int64_t ldx,
              int64_t ldr, void *h, void *y, int y_type, void *stream, bool overlap);
 int dequantize_act(int act_dtype, const void *act_blocks, int64_t elem_count, float *out, void *stream, bool overlap);
+// The microscaled 4-bit entries of the same names (mx.cu); overlap in mx_forward: the weights are in place
+int mx_quantize(const void *x, int x_type, int64_t rows, int64_t k, void *image, int64_t image_bytes, void *stream, bool overlap);
+int mx_dequantize(const void *image, int64_t rows, int64_t k, void *out, bool f16, void *stream, bool overlap);
+int mx_forward(const void *image, const void *x, int x_type, void *y, int y_type, int64_t m, int64_t n, int64_t k, int64_t ldy, void *workspace,
+               int64_t workspace_bytes, void *stream, bool overlap);
 
 }  // namespace lloom

@@ -392,6 +392,138 @@ PyObject *module_group(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
     END_HANDLE_TH_ERRORS
 }
 
+// Native half of MxTensor: the image of an [n, k] matrix of microscaled 4-bit values, which nobody else holds.
+struct MxStorage {
+    PyObject_HEAD
+    at::Tensor *image;
+    int64_t n, k;
+    bool settled;
+};
+PyTypeObject MxStorageType = {PyVarObject_HEAD_INIT(nullptr, 0)};
+
+void MxStorage_dealloc(PyObject *o) {
+    delete reinterpret_cast<MxStorage *>(o)->image;
+    Py_TYPE(o)->tp_free(o);
+}
+
+// An image of its own for [n, k], not yet written; null with an exception
+MxStorage *mx_new(int64_t n, int64_t k, c10::Device dev) {
+    PyObject *o = MxStorageType.tp_alloc(&MxStorageType, 0);
+    if (!o) return nullptr;
+    MxStorage *st = reinterpret_cast<MxStorage *>(o);
+    st->n = n;
+    st->k = k;
+    st->settled = false;
+    try {
+        st->image = new at::Tensor(at::detail::empty_cuda({lloom_b200_mx_image_bytes(n, k)}, at::kByte, dev, std::nullopt));
+    } catch (...) {
+        Py_DECREF(o);
+        throw;
+    }
+    return st;
+}
+
+cudaStream_t stream_of(c10::Device dev) { return c10::cuda::getCurrentCUDAStream(dev.index()).stream(); }
+
+// mx_quantize(x [.., k]) -> storage of [rows, k]
+PyObject *module_mx_quantize(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    int x_type;
+    if (nargs != 1 || !THPVariable_Check(args[0])) Py_RETURN_NONE;
+    at::Tensor x = THPVariable_Unpack(args[0]);
+    if (!x.defined() || !x.is_cuda() || x.layout() != at::kStrided || !elem_type(x.scalar_type(), x_type) || x.dim() < 2 || x.numel() == 0 ||
+        !x.is_contiguous())
+        Py_RETURN_NONE;
+    const int64_t k = x.size(-1), n = x.numel() / k;
+    if (lloom_b200_mx_image_bytes(n, k) <= 0) Py_RETURN_NONE;
+    const c10::Device dev = x.device();
+    c10::cuda::CUDAGuard guard(dev);
+    if (!aligned16(x.const_data_ptr())) x = x.clone();
+    MxStorage *st = mx_new(n, k, dev);
+    if (!st) return nullptr;
+    THPObjectPtr own(reinterpret_cast<PyObject *>(st));
+    const int rc = lloom::mx_quantize(x.const_data_ptr(), x_type, n, k, st->image->data_ptr(), st->image->numel(), stream_of(dev),
+                                      lloom::launch_overlap() != 0);
+    if (rc != LLOOM_OK) return fail(rc, "mx_quantize");
+    return own.release();
+    END_HANDLE_TH_ERRORS
+}
+
+// mx_from_blocks(blocks uint8 on the GPU, (n, k)) -> storage
+PyObject *module_mx_from_blocks(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    int64_t n, k;
+    if (nargs != 2 || !THPVariable_Check(args[0]) || !shape2(args[1], n, k)) return none_or_error();
+    const at::Tensor &b = THPVariable_Unpack(args[0]);
+    if (!b.defined() || !b.is_cuda() || b.scalar_type() != at::kByte || !b.is_contiguous() || lloom_b200_mx_image_bytes(n, k) <= 0 ||
+        b.numel() != n * (k / 32) * 17)
+        Py_RETURN_NONE;
+    c10::cuda::CUDAGuard guard(b.device());
+    MxStorage *st = mx_new(n, k, b.device());
+    if (!st) return nullptr;
+    THPObjectPtr own(reinterpret_cast<PyObject *>(st));
+    const int rc = lloom_b200_mx_from_blocks(b.const_data_ptr(), n, k, st->image->data_ptr(), st->image->numel(), stream_of(b.device()));
+    if (rc != LLOOM_OK) return fail(rc, "mx_from_blocks");
+    return own.release();
+    END_HANDLE_TH_ERRORS
+}
+
+// to_blocks() -> uint8 [n, k / 32 * 17] on the GPU
+PyObject *MxStorage_to_blocks(PyObject *o, PyObject *) {
+    HANDLE_TH_ERRORS
+    MxStorage *self = reinterpret_cast<MxStorage *>(o);
+    const c10::Device dev = self->image->device();
+    c10::cuda::CUDAGuard guard(dev);
+    at::Tensor out = at::detail::empty_cuda({self->n, self->k / 32 * 17}, at::kByte, dev, std::nullopt);
+    const int rc = lloom_b200_mx_to_blocks(self->image->const_data_ptr(), self->n, self->k, out.data_ptr(), stream_of(dev));
+    if (rc != LLOOM_OK) return fail(rc, "mx_to_blocks");
+    return THPVariable_Wrap(out);
+    END_HANDLE_TH_ERRORS
+}
+
+// dequantize(f16) -> [n, k]
+PyObject *MxStorage_dequantize(PyObject *o, PyObject *f16) {
+    HANDLE_TH_ERRORS
+    MxStorage *self = reinterpret_cast<MxStorage *>(o);
+    const c10::Device dev = self->image->device();
+    c10::cuda::CUDAGuard guard(dev);
+    at::Tensor out = at::detail::empty_cuda({self->n, self->k}, f16 == Py_True ? at::kHalf : at::kFloat, dev, std::nullopt);
+    const int rc = lloom::mx_dequantize(self->image->const_data_ptr(), self->n, self->k, out.data_ptr(), f16 == Py_True, stream_of(dev),
+                                        lloom::launch_overlap() != 0);
+    if (rc != LLOOM_OK) return fail(rc, "mx_dequantize");
+    return THPVariable_Wrap(out);
+    END_HANDLE_TH_ERRORS
+}
+
+// forward(x [.., k]) -> [.., n] of x's type
+PyObject *MxStorage_forward(PyObject *o, PyObject *const *args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    MxStorage *self = reinterpret_cast<MxStorage *>(o);
+    int x_type;
+    if (nargs != 1 || !THPVariable_Check(args[0])) Py_RETURN_NONE;
+    at::Tensor x = THPVariable_Unpack(args[0]);
+    const c10::Device dev = self->image->device();
+    if (!x.defined() || x.device() != dev || x.layout() != at::kStrided || !elem_type(x.scalar_type(), x_type) || x.dim() < 2 ||
+        x.size(-1) != self->k || x.numel() == 0 || !x.is_contiguous())
+        Py_RETURN_NONE;
+    c10::cuda::CUDAGuard guard(dev);
+    if (!aligned16(x.const_data_ptr())) x = x.clone();
+    const int64_t m = x.numel() / self->k, need = lloom_b200_mx_workspace_bytes(m, self->n, self->k);
+    if (need <= 0) Py_RETURN_NONE;
+    c10::SmallVector<int64_t, 5> sizes(x.sizes().begin(), x.sizes().end());
+    sizes.back() = self->n;
+    at::Tensor y = at::detail::empty_cuda(sizes, x.scalar_type(), dev, std::nullopt);
+    const cudaStream_t stream = stream_of(dev);
+    const at::Tensor &ws = workspaces().get(dev, stream, need);
+    const int mode = lloom::launch_overlap();
+    const int rc = lloom::mx_forward(self->image->const_data_ptr(), x.const_data_ptr(), x_type, y.data_ptr(), x_type, m, self->n, self->k,
+                                     self->n, ws.data_ptr(), ws.numel(), stream, mode > 0 || (mode < 0 && self->settled));
+    if (rc != LLOOM_OK) return fail(rc, "mx_fwd");
+    self->settled = true;
+    return THPVariable_Wrap(y);
+    END_HANDLE_TH_ERRORS
+}
+
 // The rows of [.., k] and how far apart they are: a contiguous tensor, or a matrix whose rows are
 bool row_layout(const at::Tensor &t, int64_t &rows, int64_t &k, int64_t &ld) {
     if (!t.defined() || t.layout() != at::kStrided || !t.is_cuda() || t.dim() < 1) return false;
@@ -499,9 +631,16 @@ PyMethodDef storage_methods[] = {{"forward", FAST(Storage_forward), METH_FASTCAL
                                  {"overlaps", Storage_overlaps, METH_NOARGS, nullptr},
                                  {nullptr, nullptr, 0, nullptr}};
 
+PyMethodDef mx_methods[] = {{"forward", FAST(MxStorage_forward), METH_FASTCALL, nullptr},
+                            {"dequantize", MxStorage_dequantize, METH_O, nullptr},
+                            {"to_blocks", MxStorage_to_blocks, METH_NOARGS, nullptr},
+                            {nullptr, nullptr, 0, nullptr}};
+
 PyMethodDef module_methods[] = {{"group", FAST(module_group), METH_FASTCALL, nullptr},
                                 {"rms_norm", FAST(module_rms_norm), METH_FASTCALL, nullptr},
                                 {"dequantize_act", FAST(module_dequantize_act), METH_FASTCALL, nullptr},
+                                {"mx_quantize", FAST(module_mx_quantize), METH_FASTCALL, nullptr},
+                                {"mx_from_blocks", FAST(module_mx_from_blocks), METH_FASTCALL, nullptr},
                                 {"workspace", module_workspace, METH_VARARGS, nullptr},
                                 {"set_error", module_set_error, METH_O, nullptr},
                                 {nullptr, nullptr, 0, nullptr}};
@@ -518,6 +657,12 @@ PyMODINIT_FUNC PyInit__native(void) {
     StorageType.tp_dealloc = Storage_dealloc;
     StorageType.tp_methods = storage_methods;
     if (PyType_Ready(&StorageType) < 0) return nullptr;
+    MxStorageType.tp_name = "lloom_b200._native.MxStorage";
+    MxStorageType.tp_basicsize = sizeof(MxStorage);
+    MxStorageType.tp_flags = Py_TPFLAGS_DEFAULT;
+    MxStorageType.tp_dealloc = MxStorage_dealloc;
+    MxStorageType.tp_methods = mx_methods;
+    if (PyType_Ready(&MxStorageType) < 0) return nullptr;
     PyObject *m = PyModule_Create(&module_def);
     if (!m) return nullptr;
     Py_INCREF(&StorageType);

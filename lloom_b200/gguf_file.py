@@ -7,8 +7,9 @@ data section from ``general.alignment`` (:638-653) -- with the reference's size 
 checks (:125-145, :664-669); ``Content.tensor`` (:671-683) reads one tensor's bytes and hands them to the device
 slot exactly as stored (``qtensor_from_ggml`` -> ``QStorage::from_data``, ggml_file.rs:180-228): the file's block
 stream IS the device layout, so ingest is one staged copy (pinned host buffer -> device), no repack.
-``write`` (:749-) is the inverse for the same subset.  Tensor types other than Q8_0 / Q4_K / Q6_K are listed by
-``read`` but refused by ``tensor``: there is no fallback path.
+``write`` (:749-) is the inverse for the same subset.  MXFP4 tensors become an ``MxTensor``, laid out for the tensor cores
+by one kernel.  Tensor types other than these and Q8_0 / Q4_K / Q6_K are listed by ``read`` but refused by ``tensor``: there is no
+fallback path.
 """
 from __future__ import annotations
 
@@ -33,8 +34,9 @@ _SCALAR = {T_U8: "<B", T_I8: "<b", T_U16: "<H", T_I16: "<h", T_U32: "<I", T_I32:
 # first three can be loaded
 _TYPE_GEOMETRY = {8: (32, 34), 12: (256, 144), 14: (256, 210),
                   0: (1, 4), 1: (1, 2), 2: (32, 18), 3: (32, 20), 6: (32, 22), 7: (32, 24), 9: (32, 36),
-                  10: (256, 84), 11: (256, 110), 13: (256, 176), 15: (256, 292), 30: (1, 2)}
+                  10: (256, 84), 11: (256, 110), 13: (256, 176), 15: (256, 292), 30: (1, 2), 39: (32, 17)}
 LOADABLE = (8, 12, 14)
+MXFP4 = 39  # loaded as an MxTensor
 
 
 class GgufError(ValueError):
@@ -97,9 +99,14 @@ class TensorInfo:
         return host
 
     def read(self, f: BinaryIO, tensor_data_offset: int, device):
-        """:147-170 -> QTensor on ``device``."""
+        """:147-170 -> QTensor on ``device`` (MxTensor for MXFP4 blocks)."""
+        from .microscaled import MxTensor
         from .quantized import GgmlDType, QTensor
 
+        if self.ggml_dtype == MXFP4:
+            if len(self.shape) != 2:
+                raise GgufError(f"gguf: microscaled tensor of rank {len(self.shape)}; the matmul takes [n, k]")
+            return MxTensor.from_data(self.read_bytes(f, tensor_data_offset), self.shape, device)
         if self.ggml_dtype not in LOADABLE:
             raise GgufError(f"gguf: ggml dtype {self.ggml_dtype} is not one of Q8_0 / Q4_K / Q6_K (no fallback path)")
         if len(self.shape) != 2:

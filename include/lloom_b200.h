@@ -54,7 +54,8 @@ enum {
     LLOOM_ERR_LAUNCH = 6,    /* CUDA reported an error at launch (see lloom_b200_last_cuda_error) */
     LLOOM_ERR_TIMEOUT = 7,   /* a bounded device-side wait ran out (reported by lloom_b200_device_status) */
     LLOOM_ERR_DEVICE = 8,    /* not an sm_100 device / attribute query failed */
-    LLOOM_ERR_STATIC_LIMIT = 9 /* request exceeds the built-in scratch of lloom_b200_qmatmul_fwd_static */
+    LLOOM_ERR_STATIC_LIMIT = 9, /* request exceeds the built-in scratch of lloom_b200_qmatmul_fwd_static */
+    LLOOM_ERR_VALUE = 10     /* a setting outside its range */
 };
 
 /* Library version (LLOOM_B200_VERSION of the build). */
@@ -254,6 +255,21 @@ int lloom_b200_mx_dequantize(const void *image, int64_t rows, int64_t k, void *o
 int64_t lloom_b200_mx_workspace_bytes(int64_t m, int64_t n, int64_t k);
 int lloom_b200_mx_fwd(const void *image, const void *x, int x_type, void *y, int y_type, int64_t m, int64_t n, int64_t k, int64_t ldy,
                       void *workspace, int64_t workspace_bytes, void *stream);
+
+/* ---- The next token of every row of logits ----
+ * w_i = exp((l_i - max) / temperature).  Tokens in the order (logit falling, index rising); kept is the shortest of three prefixes of it:
+ * the first top_k (0: all), the first whose weights reach top_p times those of the first top_k (1: all; at least one token), those with
+ * w_i >= min_p (0: all).  Drawn, of the kept tokens by rising index: the first whose running sum of weights exceeds u times their sum,
+ * 0 <= u < 1 (u >= 1: the last with a weight).  temperature 0: the first of the largest logits.  A NaN counts as -infinity;
+ * logits of +infinity share the draw.  Weights below 2^-44 of the largest are never drawn.
+ * logits: batch rows of vocab elements of `type`, ld elements apart; u f32 [batch].  Each setting is an f32 (top_k: int32) array per row on the
+ * device, or NULL and the value beside it for all rows.  Values of an array outside the range are read as the range's end (a
+ * temperature not above 0 as 0, top_k below 1 as 0), those given directly are refused (LLOOM_ERR_VALUE).
+ * ids[batch]: the token, or -1 for a row with nothing above -infinity; probs[batch] (may be NULL): its weight over that of all kept ones. */
+#define LLOOM_B200_MAX_VOCAB 327680
+int lloom_b200_sample(const void *logits, int type, int64_t batch, int64_t vocab, int64_t ld, const float *u, const float *temperature,
+                      double temperature_all, const int *top_k, int64_t top_k_all, const float *top_p, double top_p_all,
+                      const float *min_p, double min_p_all, int64_t *ids, float *probs, void *stream);
 
 /* ---- Routed mixture-of-experts forward: QCudaStorage::indexed_moe_forward (cuda.rs:505-622) ----
  * w_experts: [n_experts][n][k / block] canonical blocks (one stacked tensor, 16-byte aligned); x f32 [batch][in_dim1][k] with in_dim1 == 1 or topk; ids u32 [batch][topk] ON THE DEVICE;

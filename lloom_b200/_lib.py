@@ -11,7 +11,7 @@ import os
 _PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_PKG, "liblloom_b200.so")
 
-OK, ERR_DTYPE, ERR_SHAPE, ERR_ALIGN, ERR_NULL, ERR_WORKSPACE, ERR_LAUNCH, ERR_TIMEOUT, ERR_DEVICE, ERR_STATIC_LIMIT = range(10)
+OK, ERR_DTYPE, ERR_SHAPE, ERR_ALIGN, ERR_NULL, ERR_WORKSPACE, ERR_LAUNCH, ERR_TIMEOUT, ERR_DEVICE, ERR_STATIC_LIMIT, ERR_VALUE = range(11)
 
 # Every symbol include/lloom_b200.h declares: (name, restype, argtypes)
 _i64, _vp, _int = C.c_int64, C.c_void_p, C.c_int
@@ -66,6 +66,7 @@ SYMBOLS = [
     ("lloom_b200_mx_dequantize", _int, [_vp, _i64, _i64, _vp, _int, _vp]),
     ("lloom_b200_mx_workspace_bytes", _i64, [_i64, _i64, _i64]),
     ("lloom_b200_mx_fwd", _int, [_vp, _vp, _int, _vp, _int, _i64, _i64, _i64, _i64, _vp, _i64, _vp]),
+    ("lloom_b200_sample", _int, [_vp, _int, _i64, _i64, _i64, _vp, _vp, C.c_double, _vp, _i64, _vp, C.c_double, _vp, C.c_double, _vp, _vp, _vp]),
     # include/lloom_b200_host.h: C view of the C++ host layer
     ("lloom_b200_host_last_error", C.c_char_p, []),
     ("lloom_b200_host_quantize_rows", _int, [_int, _vp, _vp, _i64, _i64, _int]),

@@ -46,4 +46,9 @@ int mx_dequantize(const void *image, int64_t rows, int64_t k, void *out, bool f1
 int mx_forward(const void *image, const void *x, int x_type, void *y, int y_type, int64_t m, int64_t n, int64_t k, int64_t ldy, void *workspace,
                int64_t workspace_bytes, void *stream, bool overlap);
 
+// lloom_b200_sample (sample.cu)
+int sample(const void *logits, int type, int64_t batch, int64_t vocab, int64_t ld, const float *u, const float *temperature, double temperature_all,
+           const int *top_k, int64_t top_k_all, const float *top_p, double top_p_all, const float *min_p, double min_p_all, int64_t *ids,
+           float *probs, void *stream, bool overlap);
+
 }  // namespace lloom

@@ -845,6 +845,7 @@ const char *lloom_b200_error_string(int status) {
     case LLOOM_ERR_TIMEOUT: return "device-side wait timed out";
     case LLOOM_ERR_DEVICE: return "not an sm_100 device";
     case LLOOM_ERR_STATIC_LIMIT: return "request exceeds the built-in scratch (m <= 8 and m * act_row_bytes <= 256 KiB)";
+    case LLOOM_ERR_VALUE: return "setting outside its range";
     }
     return "unknown status";
 }

@@ -600,6 +600,50 @@ PyObject *module_dequantize_act(PyObject *, PyObject *const *args, Py_ssize_t na
     END_HANDLE_TH_ERRORS
 }
 
+// A setting of the sampler: one number, or a contiguous tensor with a value per row.  False with or without an exception
+bool setting(PyObject *o, const at::Tensor &like, int64_t rows, at::ScalarType type, const void *&per_row, double &all) {
+    per_row = nullptr;
+    all = 0.0;
+    if (!THPVariable_Check(o)) {
+        all = PyFloat_AsDouble(o);
+        return !PyErr_Occurred();
+    }
+    const at::Tensor &t = THPVariable_Unpack(o);
+    if (!t.defined() || t.device() != like.device() || t.scalar_type() != type || t.numel() != rows || !t.is_contiguous()) return false;
+    per_row = t.const_data_ptr();
+    return true;
+}
+
+// sample(logits [.., vocab], u, temperature, top_k, top_p, min_p) -> (ids, probs)
+PyObject *module_sample(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    if (nargs != 6 || !THPVariable_Check(args[0]) || !THPVariable_Check(args[1])) Py_RETURN_NONE;
+    const at::Tensor &x = THPVariable_Unpack(args[0]), &u = THPVariable_Unpack(args[1]);
+    int64_t rows, vocab, ld;
+    int type;
+    if (!row_layout(x, rows, vocab, ld) || !elem_type(x.scalar_type(), type)) Py_RETURN_NONE;
+    if (!u.defined() || u.device() != x.device() || u.scalar_type() != at::kFloat || u.sizes() != x.sizes().slice(0, x.dim() - 1) || !u.is_contiguous())
+        Py_RETURN_NONE;
+    const void *t, *k, *p, *mp;
+    double t_all, k_all, p_all, mp_all;
+    if (!setting(args[2], x, rows, at::kFloat, t, t_all) || !setting(args[3], x, rows, at::kInt, k, k_all) ||
+        !setting(args[4], x, rows, at::kFloat, p, p_all) || !setting(args[5], x, rows, at::kFloat, mp, mp_all))
+        return none_or_error();
+    const c10::Device dev = x.device();
+    c10::cuda::CUDAGuard guard(dev);
+    at::Tensor ids = at::detail::empty_cuda(u.sizes(), at::kLong, dev, std::nullopt), probs = at::detail::empty_cuda(u.sizes(), at::kFloat, dev, std::nullopt);
+    if (rows > 0) {
+        const int64_t k_int = k_all >= 0 ? (int64_t)std::min(k_all, 9.0e15) : -1;
+        const int rc = lloom::sample(x.const_data_ptr(), type, rows, vocab, ld, u.const_data_ptr<float>(), (const float *)t, t_all, (const int *)k,
+                                     k_int, (const float *)p, p_all, (const float *)mp, mp_all, ids.data_ptr<int64_t>(), probs.data_ptr<float>(),
+                                     stream_of(dev), lloom::launch_overlap() != 0);
+        if (rc != LLOOM_OK) return fail(rc, "sample");
+    }
+    THPObjectPtr a(THPVariable_Wrap(ids)), b(THPVariable_Wrap(probs));
+    return a && b ? PyTuple_Pack(2, a.get(), b.get()) : nullptr;
+    END_HANDLE_TH_ERRORS
+}
+
 // workspace(device index, stream, bytes) -> uint8 tensor of at least that size, kept for later calls
 PyObject *module_workspace(PyObject *, PyObject *args) {
     HANDLE_TH_ERRORS
@@ -641,6 +685,7 @@ PyMethodDef module_methods[] = {{"group", FAST(module_group), METH_FASTCALL, nul
                                 {"dequantize_act", FAST(module_dequantize_act), METH_FASTCALL, nullptr},
                                 {"mx_quantize", FAST(module_mx_quantize), METH_FASTCALL, nullptr},
                                 {"mx_from_blocks", FAST(module_mx_from_blocks), METH_FASTCALL, nullptr},
+                                {"sample", FAST(module_sample), METH_FASTCALL, nullptr},
                                 {"workspace", module_workspace, METH_VARARGS, nullptr},
                                 {"set_error", module_set_error, METH_O, nullptr},
                                 {nullptr, nullptr, 0, nullptr}};

@@ -1,0 +1,231 @@
+"""The draw of the next token against the definition in 64 bits and more: the same token, and its probability."""
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+TYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+LAST = float(np.nextafter(np.float32(1), np.float32(0)))
+
+
+@pytest.fixture(scope="module")
+def dev(cuda_lib):
+    assert torch.cuda.is_available()
+    return torch.device("cuda:0")
+
+
+def draw(l, u, t, k, p, mp):
+    """One row, from the definition: (token, probability)."""
+    l = np.where(np.isnan(l), -np.inf, l.astype(np.float64))
+    top = l.max()
+    if top == -np.inf:
+        return -1, 0.0
+    if not t > 0:
+        return int(l.argmax()), 1.0
+    order = np.argsort(-l, kind="stable")
+    with np.errstate(invalid="ignore", over="ignore"):
+        w = np.where(l == top, 1.0, np.exp((l - top) / t))
+    w = np.where(np.isnan(w), 0, w).astype(np.longdouble)
+    n = len(l) if k <= 0 else min(k, len(l))
+    sums = np.cumsum(w[order[:n]])
+    length = n
+    if p < 1:
+        length = min(n, 1 + int(np.searchsorted(sums, np.longdouble(p) * sums[-1], side="left")))
+    if mp > 0:
+        length = min(length, max(1, int((w[order[:n]] >= mp).sum())))
+    at = np.sort(order[:length])
+    sums = np.cumsum(w[at])
+    j = min(int(np.searchsorted(sums, np.longdouble(u) * sums[-1], side="right")), length - 1)
+    while w[at[j]] == 0:  # u at the end: the last with a weight
+        j -= 1
+    return int(at[j]), float(w[at[j]] / sums[-1])
+
+
+def check(dev, logits, u, t=1.0, k=0, p=1.0, mp=0.0):
+    """Tokens equal the definition's; probabilities within the rounding to f32 and of the fixed-point sum (2^-44 per token)."""
+    import lloom_b200 as lb
+
+    rows = logits.shape[0]
+    args = [torch.tensor(v, dtype=torch.int32 if i == 1 else torch.float32, device=dev) if isinstance(v, (list, np.ndarray)) else v
+            for i, v in enumerate((t, k, p, mp))]
+    u = np.asarray(u, np.float32)
+    ids, probs = lb.sample(logits.to(dev), torch.from_numpy(u).to(dev), *args)
+    assert ids.dtype == torch.int64 and probs.dtype == torch.float32 and ids.shape == (rows,)
+    ids, probs, host = ids.cpu().numpy(), probs.cpu().numpy(), logits.float().numpy()
+    per = [np.broadcast_to(np.asarray(v, np.float32 if isinstance(v, (list, np.ndarray)) else np.float64), (rows,)) for v in (t, k, p, mp)]
+    for i in range(rows):
+        want, prob = draw(host[i], np.float64(u[i]), np.float64(per[0][i]), int(per[1][i]), np.float64(per[2][i]), np.float64(per[3][i]))
+        assert ids[i] == want, (i, ids[i], want, prob)
+        assert abs(probs[i] - prob) <= prob * (2.0 ** -24 + host.shape[1] * 2.0 ** -44 + 1e-12), (i, probs[i], prob)
+
+
+def rand(seed, b, v, dtype=torch.float32, scale=2.5):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(b, v, generator=g) * scale
+    x.scatter_add_(1, torch.randint(0, v, (b, min(v, 24)), generator=g), 4 + 3 * torch.randn(b, min(v, 24), generator=g).abs())
+    return x.to(dtype), torch.rand(b, generator=g).numpy()
+
+
+SETTINGS = [dict(), dict(t=0.7), dict(k=1), dict(k=40, p=0.95, mp=0.05, t=0.8), dict(p=0.9), dict(p=0.999, t=1.5), dict(mp=0.02), dict(k=300, p=0.5),
+            dict(k=2000, t=2.0), dict(k=2000, p=0.99, t=2.0), dict(p=0.0), dict(t=0.0), dict(t=50.0), dict(t=50.0, p=0.7), dict(t=50.0, k=777, p=0.9), dict(t=1e-3, k=5)]
+
+
+@pytest.mark.parametrize("x", TYPES)
+@pytest.mark.parametrize("v", [1, 2, 31, 1000, 4096, 4097, 32769, 50257])
+def test_settings(dev, v, x):
+    for i, s in enumerate(SETTINGS):
+        logits, u = rand(v + i, 5, v, TYPES[x])
+        check(dev, logits, u, **s)
+
+
+@pytest.mark.parametrize("x", TYPES)
+@pytest.mark.parametrize("v", [128256, 327680])
+def test_large(dev, v, x):
+    for i, s in enumerate(SETTINGS):
+        logits, u = rand(v + i, 2, v, TYPES[x])
+        check(dev, logits, u, **s)
+
+
+@pytest.mark.parametrize("v", [64, 5000, 40000])
+def test_equal_logits(dev, v):
+    """All equal, and two values only: more ties than are ranked; the filters cut by index."""
+    u = np.linspace(0, LAST, 7).astype(np.float32)
+    flat = torch.full((7, v), -1.25)
+    two = torch.where(torch.rand(7, v, generator=torch.Generator().manual_seed(1)) < 0.5, 1.0, 0.25)
+    for logits in (flat, two):
+        for s in (dict(), dict(k=v // 3), dict(p=0.37), dict(k=v // 2 + 1, p=0.8), dict(t=0.0), dict(mp=1.0), dict(k=3), dict(p=0.9, t=0.01)):
+            check(dev, logits, u, **s)
+
+
+def test_close_logits(dev):
+    """Values one unit in the last place apart around zero and far from it: one bucket holds them all, their bits tell them apart."""
+    v = 9000
+    g = torch.Generator().manual_seed(2)
+    near = torch.randn(3, v, generator=g) * 1e-4
+    far = 100 + torch.randint(0, 600, (3, v), generator=g) * 2.0 ** -17
+    for logits in (near, far):
+        for s in (dict(k=500), dict(p=0.31), dict(k=5000, p=0.5), dict(k=8999)):
+            check(dev, logits, np.array([0.1, 0.5, 0.93]), **s)
+
+
+def test_masks_and_specials(dev):
+    """-infinity, the type's lowest value, NaN, +infinity, rows with one token and with none."""
+    v = 5000
+    logits, u = rand(3, 12, v)
+    logits[0, 10:] = -float("inf")
+    logits[1, ::2] = torch.finfo(torch.float32).min
+    logits[2] = -float("inf")
+    logits[3] = -float("inf")
+    logits[3, 4999] = -7.0
+    logits[4, 100] = float("nan")
+    logits[5] = float("nan")
+    logits[6, [7, 70, 700]] = float("inf")
+    logits[7] = torch.finfo(torch.float32).min
+    logits[8, 1:] = torch.finfo(torch.float32).min
+    logits[9] = torch.finfo(torch.float32).max
+    logits[10, 3] = torch.finfo(torch.float32).max
+    for s in (dict(), dict(t=0.0), dict(k=3), dict(k=4000, p=0.9), dict(p=0.5), dict(mp=0.1), dict(k=20, p=0.8, mp=0.01, t=0.3)):
+        check(dev, logits, u, **s)
+    low = logits.half()
+    low[1, ::2] = torch.finfo(torch.float16).min
+    check(dev, low, u, k=100, p=0.9)
+
+
+def test_uniform_numbers_at_the_ends(dev):
+    logits, _ = rand(4, 4, 3000)
+    for s in (dict(), dict(k=17), dict(p=0.6)):
+        check(dev, logits, np.array([0.0, LAST, 1e-30, 0.5]), **s)
+    import lloom_b200 as lb
+
+    ids, _ = lb.sample(logits.to(dev), torch.tensor([1.0, 5.0, float("nan"), -1.0], device=dev), top_k=9)
+    kept = [sorted(np.argsort(-logits[i].numpy(), kind="stable")[:9]) for i in range(4)]
+    assert ids.tolist() == [kept[0][-1], kept[1][-1], kept[2][0], kept[3][0]]
+
+
+def test_settings_per_row(dev):
+    b, v = 24, 20000
+    logits, u = rand(5, b, v)
+    rng = np.random.default_rng(0)
+    t = rng.uniform(0.2, 2.0, b).astype(np.float32)
+    t[3] = 0
+    k = rng.integers(0, 400, b).astype(np.int32)
+    k[[1, 2]] = [0, v + 5]
+    p = rng.uniform(0.3, 1.0, b).astype(np.float32)
+    p[4] = 1.0
+    mp = (rng.uniform(0, 0.1, b) * (rng.random(b) < 0.5)).astype(np.float32)
+    check(dev, logits, u, t, k, p, mp)
+    check(dev, logits, u, t=t, p=0.9)
+    # outside the range: the range's end
+    check(dev, logits[:4], u[:4], t=np.array([-1.0, 1.0, 1.0, 1.0], np.float32), k=np.array([3, -7, 0, 2], np.int32),
+          p=np.array([0.5, 2.0, -1.0, 0.5], np.float32), mp=np.array([0, 0, -3.0, 0], np.float32))
+
+
+def test_frequencies(dev):
+    """Evenly spaced uniform numbers draw every token as often as its probability says, to within one draw."""
+    import lloom_b200 as lb
+
+    v, n = 50, 4096
+    row = torch.randn(v, generator=torch.Generator().manual_seed(6))
+    u = (torch.arange(n) + 0.5) / n
+    ids, _ = lb.sample(row.expand(n, v).contiguous().to(dev), u.to(dev), temperature=0.9)
+    got = torch.bincount(ids.cpu(), minlength=v).double()
+    want = torch.softmax(row.double() / 0.9, 0) * n
+    assert ((got - want).abs() <= 1).all()
+
+
+def test_rows_apart_shapes_and_streams(dev):
+    import lloom_b200 as lb
+
+    logits, u = rand(7, 6, 3001, torch.bfloat16)
+    wide = torch.zeros(6, 5000, dtype=torch.bfloat16, device=dev)
+    wide[:, 7:3008] = logits.to(dev)
+    ud = torch.from_numpy(u).to(dev)
+    want = lb.sample(logits.to(dev), ud, 0.9, 50, 0.9)
+    got = lb.sample(wide[:, 7:3008], ud, 0.9, 50, 0.9)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    three = lb.sample(logits.to(dev).view(2, 3, 3001), ud.view(2, 3), 0.9, 50, 0.9)
+    assert three[0].shape == (2, 3) and torch.equal(three[0].view(-1), want[0])
+    one = lb.sample(logits[0].to(dev), ud[0], 0.9, 50, 0.9)
+    assert one[0].shape == () and one[0] == want[0][0]
+    none = lb.sample(torch.empty(0, 10, device=dev), torch.empty(0, device=dev))
+    assert none[0].shape == (0,)
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s):
+        got = lb.sample(logits.to(dev), ud, 0.9, 50, 0.9)
+    s.synchronize()
+    assert torch.equal(got[0], want[0])
+
+
+def test_output_head_then_draw_captured(dev):
+    """The output head's product and the draw behind it in one graph, replayed with other hidden states and numbers."""
+    import lloom_b200 as lb
+    from lloom_b200.quantized import quantize_weights_host
+
+    v, h, b = 8000, 512, 3
+    rng = np.random.default_rng(1)
+    w = quantize_weights_host(rng.standard_normal((v, h)).astype(np.float32) * np.float32(0.1), 14)
+    head = lb.QMatMul.from_qtensor(lb.QTensor.from_data(w, lb.GgmlDType.Q6K, (v, h), dev))
+    norm = torch.ones(h, device=dev)
+    x, u = torch.randn(b, h, device=dev), torch.rand(b, device=dev)
+
+    def step():
+        logits = head.forward_quantized(lb.rms_norm(x, norm, act_for=lb.GgmlDType.Q6K))
+        return lb.sample(logits, u, 0.8, 100, 0.9), logits
+
+    step()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        (ids, probs), logits = step()
+    for i in range(3):
+        x.copy_(torch.randn(b, h, device=dev))
+        u.copy_(torch.rand(b, device=dev))
+        g.replay()
+        torch.cuda.synchronize()
+        got = (ids.clone(), probs.clone())
+        (want, want_p), _ = step()
+        assert torch.equal(got[0], want) and torch.equal(got[1], want_p)
+        for r in range(b):
+            assert got[0][r] == draw(logits[r].cpu().numpy(), float(u[r]), 0.8, 100, 0.9, 0.0)[0]

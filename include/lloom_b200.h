@@ -260,7 +260,7 @@ int lloom_b200_mx_fwd(const void *image, const void *x, int x_type, void *y, int
  * w_i = exp((l_i - max) / temperature).  Tokens in the order (logit falling, index rising); kept is the shortest of three prefixes of it:
  * the first top_k (0: all), the first whose weights reach top_p times those of the first top_k (1: all; at least one token), those with
  * w_i >= min_p (0: all).  Drawn, of the kept tokens by rising index: the first whose running sum of weights exceeds u times their sum,
- * 0 <= u < 1 (u >= 1: the last with a weight).  temperature 0: the first of the largest logits.  A NaN counts as -infinity;
+ * 0 <= u < 1 (u >= 1: the last with a weight).  temperature 0 (and below 2^-120): the first of the largest logits.  A NaN counts as -infinity;
  * logits of +infinity share the draw.  Weights below 2^-44 of the largest are never drawn.
  * logits: batch rows of vocab elements of `type`, ld elements apart; u f32 [batch].  Each setting is an f32 (top_k: int32) array per row on the
  * device, or NULL and the value beside it for all rows.  Values of an array outside the range are read as the range's end (a

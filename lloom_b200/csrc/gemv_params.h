@@ -151,6 +151,9 @@ __host__ __device__ inline int64_t bank_pitch(int64_t bytes, int unit) {
     return q * unit * 4;
 }
 
+// TMA map of n rows of row_bytes (a multiple of 16): boxes of box_rows x width bytes (lloom_b200.cu); false: the driver refused
+bool encode_rows_map(CUtensorMap &map, const void *w, int64_t n, int64_t row_bytes, int64_t width, int box_rows);
+
 // ---- launchers exported by the kernels' translation units ----
 // dp4a GEMV, one unit per weight format.  rw: rows per lane (1 or 2).
 cudaError_t launch_gemv_dp4a_q8_0(const GemvParams &p, dim3 grid, int smem, bool overlap, int rw, cudaStream_t stream);

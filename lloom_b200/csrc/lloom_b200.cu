@@ -327,9 +327,9 @@ static int64_t staging_bytes(int n_peers, int64_t m, int64_t rows_per_cta, int &
     return bytes <= 32 * 1024 ? bytes : 0;
 }
 
-// TMA view of the packed rows: boxes of 16 rows x `width` bytes, what lies past the matrix reads as zero.  (The driver's
+// TMA view of rows of bytes: boxes of `box_rows` rows x `width` bytes, what lies past the matrix reads as zero.  (The driver's
 // encoder is host arithmetic, 40 ns a call, so nothing is cached.)
-static bool encode_rows_map(CUtensorMap &map, const void *w, int64_t n, int64_t row_bytes, int64_t width) {
+bool encode_rows_map(CUtensorMap &map, const void *w, int64_t n, int64_t row_bytes, int64_t width, int box_rows) {
     using Encode = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
                                 const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -341,7 +341,7 @@ static bool encode_rows_map(CUtensorMap &map, const void *w, int64_t n, int64_t 
     }();
     if (!encode) return false;
     const cuuint64_t dims[2] = {(cuuint64_t)row_bytes / 8, (cuuint64_t)n}, stride[1] = {(cuuint64_t)row_bytes};
-    const cuuint32_t box[2] = {(cuuint32_t)width / 8, (cuuint32_t)kMmaTileRows}, step[2] = {1, 1};
+    const cuuint32_t box[2] = {(cuuint32_t)width / 8, (cuuint32_t)box_rows}, step[2] = {1, 1};
     return encode(&map, CU_TENSOR_MAP_DATA_TYPE_FLOAT64, 2, const_cast<void *>(w), dims, stride, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
                   CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
@@ -390,7 +390,7 @@ static int mma_launch(int w_dtype, const void *w, MmaActSource source, const voi
     const int smem = (int)(kMmaBarBytes + pl.red + pl.resident + out_bytes + pl.stages * pl.stage + kMmaSlack);
     CUtensorMap map;
     memset(&map, 0, sizeof(map));
-    if (pl.boxes && !encode_rows_map(map, w, n, p.row_bytes, pl.pitch)) return LLOOM_ERR_DEVICE;
+    if (pl.boxes && !encode_rows_map(map, w, n, p.row_bytes, pl.pitch, kMmaTileRows)) return LLOOM_ERR_DEVICE;
     return launch_status(launch_mma(p, map, pl.nt, pl.grid_x, pl.grid_y, smem, io.overlap, stream));
 }
 

@@ -13,6 +13,7 @@
 //                    then per 128 rows two scale atoms of 512 bytes (128 elements of K each): scale of row r, block b at
 //                    (r % 32) * 16 + (r / 32) * 4 + b, the order in which tcgen05.cp spreads them over tensor memory.
 // 4.25 bits an element; K is padded to 256 and rows to the tile with zeros.
+#include <algorithm>
 #include <mutex>
 
 #include "abi.h"
@@ -412,14 +413,248 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx_gemm_kernel(const __grid_con
     }
 }
 
-// How m activation rows are cut: equal tiles of at most 256, each a multiple of 16 (of m alone, so that the image does not depend on the weights)
+// ---- product of many rows: pairs of CTAs ----
+// Two CTAs on neighbouring SMs compute a 256 x bn tile with one instruction (cta_group::2): each has 128 rows of weights and of the
+// accumulator and half of the activation rows, so that a stage brings 35 KB per CTA where one alone would load 50 for the same work: bulk copies
+// from L2 run at 69 bytes a clock and SM, and a stage of bn = 240 takes the tensor cores 480 clocks.  Persistent: the pairs walk the
+// tiles, and with two accumulators in tensor memory the stores of one tile run under the next one's products.
+// The first CTA of a pair issues the MMAs of both, and both CTAs' copies complete on its barriers, which takes TMA's tensor copies: untiled ones
+// may only signal their own CTA, and passing that on by a thread (wait, arrive across the cluster) cost a microsecond a stage, four times
+// the stage's work.  The maps see an image as rows of 128 bytes.
+constexpr int kPairMaxBn = 240;  // two accumulators and the scales fill the 512 columns
+constexpr int kPairStages = 6;
+constexpr int kPairEpiWarps = 8;
+constexpr int kPairThreads = 32 * (kPairEpiWarps + 2);
+
+struct MxPairParams {
+    CUtensorMap w, codes, scales;  // boxes of a unit's rows of 128 bytes: of weights; of half of the activations' codes; of their scales
+    void *y;
+    int y_type;
+    int64_t ldy;
+    int m, n, units;
+    int bn, m_tiles, n_tiles;  // n_tiles of 128 rows; a pair takes two
+    int stages, stage_bytes;
+};
+
+__device__ __forceinline__ uint32_t mapa(uint32_t smem, int rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem), "r"(rank));
+    return r;
+}
+// Rows `row` .. of a map's box to this CTA's shared memory; `bar`: of either CTA of the pair
+__device__ __forceinline__ void copy_rows(void *dst, const CUtensorMap *map, int row, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3}], [%4];" ::"r"(smem_u32(dst)),
+        "l"(map), "r"(0), "r"(row), "r"(bar)
+        : "memory");
+}
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void umma2_mxf4(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        ".reg .b64 da, db;\n\t"
+        "setp.ne.b32 p, %7, 0;\n\t"
+        "mov.b64 da, {%1, %3};\n\t"
+        "mov.b64 db, {%2, %3};\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], da, db, %4, [%5], [%6], p;\n\t"
+        "}\n" ::"r"(d),
+        "r"(a_lo), "r"(b_lo), "r"(kUmmaDescHiSw128), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+        : "memory");
+}
+// In both CTAs, from each one's own shared memory
+__device__ __forceinline__ void copy_scales2(uint32_t tmem, uint32_t smem_lo) {
+    asm volatile(
+        "{\n\t"
+        ".reg .b64 d;\n\t"
+        "mov.b64 d, {%1, %2};\n\t"
+        "tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], d;\n\t"
+        "}\n" ::"r"(tmem),
+        "r"(smem_lo), "r"(kDescHiScales)
+        : "memory");
+}
+// Arrives at the barrier of this address in both CTAs once the MMAs issued so far have finished
+__device__ __forceinline__ void umma2_commit(uint64_t *bar) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)),
+                 "h"((unsigned short)3)
+                 : "memory");
+}
+
+__global__ void __launch_bounds__(kPairThreads, 1) mx_gemm_pair_kernel(const __grid_constant__ MxPairParams p) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    uint64_t *full = reinterpret_cast<uint64_t *>(smem + p.stages * p.stage_bytes), *empty = full + kPairStages;
+    uint64_t *acc_full = empty + kPairStages, *acc_empty = acc_full + 2;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(acc_empty + 2);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = blockIdx.x & 1;
+    const int tiles = (p.n_tiles + 1) / 2 * p.m_tiles, first = blockIdx.x >> 1, step = gridDim.x >> 1;
+    constexpr int kABytes = mx_unit_bytes(kMxTile);
+    const int half = p.bn / 2 * 128, scales = mx_scale_bytes(p.bn), unit_rows = p.bn + scales / 128;
+
+    launch_dependents();
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < p.stages; ++s) {
+            mbar_init(&full[s], 1);  // the first CTA's are used: both CTAs' copies
+            mbar_init(&empty[s], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&acc_full[i], 1);
+            mbar_init(&acc_empty[i], 2 * kPairEpiWarps);
+        }
+        *abort_flag = 0;
+        fence_mbar_init();
+    }
+    if (warp == kPairEpiWarps + 1) {
+        wait_predecessor();  // see mx_gemm_kernel
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_arrive();
+    cluster_wait();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    wait_predecessor();
+
+    if (warp == kPairEpiWarps) {
+        // ---- operand tiles ----
+        if (lane == 0) {
+            bool ok = true;
+            int s = 0, fill = 0;
+            uint32_t par = 1;
+            const uint32_t full0 = mapa(smem_u32(full), 0);
+            for (int t = first; t < tiles && ok; t += step) {
+                const int mt = t % p.m_tiles, nt = min(t / p.m_tiles * 2 + rank, p.n_tiles - 1);  // an odd last tile: once more, not stored
+                int w = nt * p.units * (kABytes / 128), a = mt * p.units * unit_rows;  // rows of 128 bytes
+                for (int u = 0; u < p.units; ++u) {
+                    if (fill >= p.stages) {
+                        ok = mbar_wait_abortable<0>(&empty[s], par, abort_flag);
+                        if (!ok) break;
+                    } else {
+                        ++fill;
+                    }
+                    uint8_t *dst = smem + s * p.stage_bytes;
+                    const uint32_t bar = full0 + 8u * (uint32_t)s;
+                    if (rank == 0) mbar_arrive_expect_tx(&full[s], (uint32_t)(2 * (kABytes + half + scales)));
+                    copy_rows(dst, &p.w, w, bar);
+                    copy_rows(dst + kABytes, &p.codes, a + rank * (p.bn / 2), bar);
+                    copy_rows(dst + kABytes + half, &p.scales, a + p.bn, bar);
+                    w += kABytes / 128;
+                    a += unit_rows;
+                    if (++s == p.stages) {
+                        s = 0;
+                        par ^= 1;
+                    }
+                }
+            }
+        }
+        __syncwarp();
+    } else if (warp == kPairEpiWarps + 1) {
+        // ---- MMA, for both CTAs ----
+        if (rank == 0 && elect_one()) {
+            const int groups = (p.bn + 127) / 128;
+            const uint32_t sfa = tmem + 2 * (uint32_t)p.bn, sfb = sfa + 8;
+            const uint32_t idesc = (1u << 7) | (1u << 10) | ((uint32_t)(p.bn >> 3) << 17) | (1u << 23) | (2u << 27);
+            const uint32_t base = smem_u32(smem);
+            bool ok = true;
+            int s = 0, acc = 0;
+            uint32_t par = 0, acc_par = 1;
+            for (int t = first; t < tiles && ok; t += step) {
+                ok = mbar_wait_abortable<0>(&acc_empty[acc], acc_par, abort_flag);
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t d = tmem + (uint32_t)(acc * p.bn);
+                for (int u = 0; u < p.units; ++u) {
+                    ok = mbar_wait_abortable<0>(&full[s], par, abort_flag);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint32_t at = base + (uint32_t)(s * p.stage_bytes), bt = at + kABytes;
+                    const uint32_t sa = umma_desc_lo(at + kMxTile * 128, 128), sb = umma_desc_lo(bt + (uint32_t)half, 128);
+                    const uint32_t a_lo = umma_desc_lo(at, 16), b_lo = umma_desc_lo(bt, 16);
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        copy_scales2(sfa + 4 * j, sa + j * (512 >> 4));
+                        copy_scales2(sfb + 8 * j, sb + j * (512 >> 4));
+                        if (groups == 2) copy_scales2(sfb + 8 * j + 4, sb + (1024 >> 4) + j * (512 >> 4));
+                    }
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const uint32_t ids = (j & 1) ? (2u << 4) | (2u << 29) : 0u;
+                        umma2_mxf4(d, a_lo + 2 * j, b_lo + 2 * j, idesc | ids, sfa + 4 * (j >> 1), sfb + 8 * (j >> 1), u > 0 || j > 0 ? 1u : 0u);
+                    }
+                    umma2_commit(&empty[s]);
+                    if (++s == p.stages) {
+                        s = 0;
+                        par ^= 1;
+                    }
+                }
+                umma2_commit(&acc_full[acc]);
+                if (acc == 1) acc_par ^= 1;
+                acc ^= 1;
+            }
+        }
+        __syncwarp();
+    } else {
+        // ---- epilogue: a warp has 32 rows of weights and about half of the columns ----
+        const int q = warp & 3, c_mid = (p.bn / 2 + 15) / 16 * 16;
+        const int c_begin = warp < 4 ? 0 : c_mid, c_end = warp < 4 ? c_mid : p.bn;
+        const uint32_t empty0 = mapa(smem_u32(acc_empty), 0);
+        bool ok = true;
+        int acc = 0;
+        uint32_t par = 0;
+        for (int t = first; t < tiles && ok; t += step) {
+            ok = mbar_wait_abortable<64>(&acc_full[acc], par, abort_flag);
+            if (!ok) break;
+            tc_fence_after();
+            const int mt = t % p.m_tiles;
+            const int64_t n = ((int64_t)(t / p.m_tiles) * 2 + rank) * kMxTile + q * 32 + lane;
+            const uint32_t from = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * p.bn);
+            with_y_type(p.y, p.y_type, [&](auto *y) {
+                for (int c = c_begin; c < c_end; c += 16) {
+                    uint32_t v[16];
+                    tmem_ld16(from + (uint32_t)c, v);
+                    tmem_ld_wait();
+                    loaded(v);
+                    const int row = mt * p.bn + c, left = p.m - row;
+                    auto *at = y + (int64_t)row * p.ldy + n;
+                    if (n < p.n) {
+#pragma unroll
+                        for (int j = 0; j < 16; ++j)
+                            if (j < left) put_y(at + (int64_t)j * p.ldy, 0, __uint_as_float(v[j]));
+                    }
+                }
+            });
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(empty0 + 8u * (uint32_t)acc);
+            if (acc == 1) par ^= 1;
+            acc ^= 1;
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_arrive();
+    cluster_wait();  // neither reads the other's memory, or computes into it, any more
+    if (warp == kPairEpiWarps + 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
+    }
+}
+
+// Activation rows in `count` equal tiles, each a multiple of 16
 struct MxTiles {
     int bn, count;
 };
-MxTiles mx_tiles(int64_t m) {
+MxTiles mx_tiles(int64_t m, int64_t count) {
     MxTiles t;
-    t.count = (int)((m + 255) / 256);
-    t.bn = (int)((m + t.count - 1) / t.count + 15) / 16 * 16;
+    t.count = (int)count;
+    t.bn = (int)((m + count - 1) / count + 15) / 16 * 16;
     return t;
 }
 
@@ -439,13 +674,49 @@ int launch_mx_quantize(const void *x, int x_type, int64_t m, int64_t k, int T, u
                                       image, trigger ? 1 : 0));
 }
 
+// Tiles for pairs of CTAs: of the widths that fit, the one with the least time over the rounds that the pairs make, a unit of K taking
+// 2 bn clocks of the tensor cores or its bytes at 69 per clock.
+MxTiles mx_pair_tiles(int64_t m, int64_t n, int pairs) {
+    const int64_t n_pairs = (n + 2 * kMxTile - 1) / (2 * kMxTile);
+    MxTiles best = {0, 0};
+    double least = 0;
+    const int64_t fewest = (m + kPairMaxBn - 1) / kPairMaxBn;
+    for (int64_t count = fewest; count < fewest + 8 && count <= (m + 63) / 64; ++count) {
+        const MxTiles t = mx_tiles(m, count);
+        const double clocks = 2.0 * t.bn, bytes = (mx_unit_bytes(kMxTile) + t.bn * 64 + mx_scale_bytes(t.bn)) / 69.0;
+        const double time = (double)((n_pairs * t.count + pairs - 1) / pairs) * (clocks > bytes ? clocks : bytes);
+        if (best.count == 0 || time < least) {
+            best = t;
+            least = time;
+        }
+    }
+    return best;
+}
+
+struct MxPlan {
+    bool pairs;
+    MxTiles tiles;
+};
+MxPlan mx_plan(int64_t m, int64_t n, int64_t k, int sms) {
+    MxPlan pl;
+    pl.pairs = m > 128;
+    pl.tiles = pl.pairs ? mx_pair_tiles(m, n, sms / 2) : mx_tiles(m, (m + 255) / 256);
+    return pl;
+}
+// Bytes of the activation image, whatever the device's plan: the largest of all tile widths
+int64_t mx_act_bytes(int64_t m, int64_t k) {
+    int64_t most = 0;
+    for (int T = 16; T <= 256; T += 16) most = std::max(most, (m + T - 1) / T * mx_unit_bytes(T));
+    return most * mx_units(k);
+}
+
 struct MxSmemOnce {
     std::mutex mu;
     bool done[64] = {false};
 };
 
-int launch_mx_gemm(const MxParams &p, int ctas, cudaStream_t stream) {
-    static MxSmemOnce once;
+template <class Params>
+int launch_mx_gemm(void (*kern)(Params), MxSmemOnce &once, const Params &p, int ctas, int cluster, int threads, cudaStream_t stream) {
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess || dev < 0 || dev >= 64) return LLOOM_ERR_DEVICE;
@@ -453,26 +724,26 @@ int launch_mx_gemm(const MxParams &p, int ctas, cudaStream_t stream) {
     {
         std::lock_guard<std::mutex> lock(once.mu);
         if (!once.done[dev]) {
-            e = cudaFuncSetAttribute(mx_gemm_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+            e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
             if (e != cudaSuccess) return launch_status(e);
             once.done[dev] = true;
         }
     }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)ctas);
-    cfg.blockDim = dim3(kMxThreads);
+    cfg.blockDim = dim3((unsigned)threads);
     cfg.dynamicSmemBytes = (size_t)smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = (unsigned)p.split;
+    attr[1].val.clusterDim.x = (unsigned)cluster;
     attr[1].val.clusterDim.y = 1;
     attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    return launch_status(cudaLaunchKernelEx(&cfg, mx_gemm_kernel, p));
+    return launch_status(cudaLaunchKernelEx(&cfg, kern, p));
 }
 
 }  // namespace
@@ -489,10 +760,39 @@ int mx_forward(const void *image, const void *x, int x_type, void *y, int y_type
     DeviceInfo di;
     rc = device_info(di);
     if (rc != LLOOM_OK) return rc;
-    const MxTiles t = mx_tiles(m);
+    const MxPlan pl = mx_plan(m, n, k, di.sm_count);
+    const MxTiles t = pl.tiles;
     // The product starts on the weights while this kernel runs, so it is not launched early itself unless they are in place.
     rc = launch_mx_quantize(x, x_type, m, k, t.bn, (uint8_t *)workspace, true, overlap, (cudaStream_t)stream);
     if (rc != LLOOM_OK) return rc;
+    const int64_t n_tiles = (n + kMxTile - 1) / kMxTile;
+    const int units = (int)mx_units(k);
+    if (pl.pairs) {
+        static MxSmemOnce once;
+        MxPairParams p = {};
+        const int64_t w_rows = mx_image_bytes(n, k, kMxTile) / 128, a_rows = mx_image_bytes(m, k, t.bn) / 128;
+        if (w_rows > 0x7fffffff || a_rows > 0x7fffffff) return LLOOM_ERR_SHAPE;  // 256 GB
+        if (!encode_rows_map(p.w, image, w_rows, 128, 128, mx_unit_bytes(kMxTile) / 128) || !encode_rows_map(p.codes, workspace, a_rows, 128, 128, t.bn / 2) ||
+            !encode_rows_map(p.scales, workspace, a_rows, 128, 128, mx_scale_bytes(t.bn) / 128))
+            return LLOOM_ERR_DEVICE;
+        p.y = y;
+        p.y_type = y_type;
+        p.ldy = ldy;
+        p.m = (int)m;
+        p.n = (int)n;
+        p.units = units;
+        p.bn = t.bn;
+        p.m_tiles = t.count;
+        p.n_tiles = (int)n_tiles;
+        p.stage_bytes = mx_unit_bytes(kMxTile) + t.bn * 64 + mx_scale_bytes(t.bn);
+        p.stages = (di.max_smem_optin - 256 - 1024) / p.stage_bytes;
+        if (p.stages > kPairStages) p.stages = kPairStages;
+        const int64_t tiles = (n_tiles + 1) / 2 * t.count;
+        if (tiles > 0x3fffffff) return LLOOM_ERR_SHAPE;
+        const int pairs = (int)(tiles < di.sm_count / 2 ? tiles : di.sm_count / 2);
+        return launch_mx_gemm(mx_gemm_pair_kernel, once, p, 2 * pairs, 2, kPairThreads, (cudaStream_t)stream);
+    }
+    static MxSmemOnce once;
     MxParams p = {};
     p.w = (const uint8_t *)image;
     p.a = (const uint8_t *)workspace;
@@ -501,10 +801,10 @@ int mx_forward(const void *image, const void *x, int x_type, void *y, int y_type
     p.ldy = ldy;
     p.m = (int)m;
     p.n = (int)n;
-    p.units = (int)mx_units(k);
+    p.units = units;
     p.bn = t.bn;
     p.m_tiles = t.count;
-    const int64_t tiles = (n + kMxTile - 1) / kMxTile * t.count;
+    const int64_t tiles = n_tiles * t.count;
     p.split = 1;
     while (p.split < 8 && tiles * p.split * 2 <= di.sm_count && p.units >= p.split * 2) p.split *= 2;
     if (tiles * p.split > 0x7fffffff) return LLOOM_ERR_SHAPE;
@@ -513,7 +813,7 @@ int mx_forward(const void *image, const void *x, int x_type, void *y, int y_type
     if (p.stages > kMxMaxStages) p.stages = kMxMaxStages;
     const int cols = (t.bn + 31) / 32 * 32 + 8 + 8 * ((t.bn + 127) / 128);
     for (p.tmem_cols = 32; p.tmem_cols < cols; p.tmem_cols *= 2) {}
-    return launch_mx_gemm(p, (int)(tiles * p.split), (cudaStream_t)stream);
+    return launch_mx_gemm(mx_gemm_kernel, once, p, (int)(tiles * p.split), p.split, kMxThreads, (cudaStream_t)stream);
 }
 
 int mx_quantize(const void *x, int x_type, int64_t rows, int64_t k, void *image, int64_t image_bytes, void *stream, bool overlap) {
@@ -546,7 +846,7 @@ extern "C" {
 int64_t lloom_b200_mx_image_bytes(int64_t rows, int64_t k) { return mx_check(1, rows, k) != LLOOM_OK ? 0 : mx_image_bytes(rows, k, kMxTile); }
 
 int64_t lloom_b200_mx_workspace_bytes(int64_t m, int64_t n, int64_t k) {
-    return mx_check(m, n, k) != LLOOM_OK ? 0 : mx_image_bytes(m, k, mx_tiles(m).bn);
+    return mx_check(m, n, k) != LLOOM_OK ? 0 : mx_act_bytes(m, k);
 }
 
 int lloom_b200_mx_quantize(const void *x, int x_type, int64_t rows, int64_t k, void *image, int64_t image_bytes, void *stream) {

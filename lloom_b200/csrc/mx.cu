@@ -12,7 +12,8 @@
 //   unit (tile, u)   T x 128 bytes of codes, K-major, 16-byte chunks (one block each) XOR-swizzled within groups of eight rows,
 //                    then per 128 rows two scale atoms of 512 bytes (128 elements of K each): scale of row r, block b at
 //                    (r % 32) * 16 + (r / 32) * 4 + b, the order in which tcgen05.cp spreads them over tensor memory.
-// 4.25 bits an element; K is padded to 256 and rows to the tile with zeros.
+// 4.25 bits an element; K is padded to 256 and rows to the tile with zeros.  Activations for pairs of CTAs: a unit is two parts, each with the
+// codes of half of the rows and the scales of all, so that a CTA of the pair copies one piece.
 #include <algorithm>
 #include <mutex>
 
@@ -33,71 +34,89 @@ constexpr int kMxBlock = 32, kMxUnit = 256, kMxBlockBytes = 17;
 constexpr int kMxTile = 128;  // weight rows per tile: the MMA's M
 
 __host__ __device__ constexpr int mx_scale_bytes(int rows) { return (rows + 127) / 128 * 1024; }
-__host__ __device__ constexpr int mx_unit_bytes(int rows) { return rows * 128 + mx_scale_bytes(rows); }
+__host__ __device__ constexpr int mx_unit_bytes(int rows, int parts = 1) { return rows * 128 + parts * mx_scale_bytes(rows); }
 __host__ __device__ inline int64_t mx_units(int64_t k) { return (k + kMxUnit - 1) / kMxUnit; }
 // offsets inside a unit of T rows: 16-byte chunk `c` (block of the unit) of row r, and the scale of that block
 __host__ __device__ inline int mx_chunk_offset(int r, int c) { return (r >> 3) * 1024 + (r & 7) * 128 + ((c ^ (r & 7)) << 4); }
-__host__ __device__ inline int mx_scale_offset(int T, int r, int c) {
-    return T * 128 + (r >> 7) * 1024 + (c >> 2) * 512 + (r & 31) * 16 + ((r >> 5) & 3) * 4 + (c & 3);
+__host__ __device__ inline int mx_scale_offset(int rows, int r, int c) {  // rows: of codes in front of the scales
+    return rows * 128 + (r >> 7) * 1024 + (c >> 2) * 512 + (r & 31) * 16 + ((r >> 5) & 3) * 4 + (c & 3);
 }
 
 // ---- quantisation ----
 
+// The larger one, or NaN if either is
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
 // Four lanes share a block, eight elements each: the lane's codes (element i in bits 4i ..) and the block's scale byte.
 __device__ __forceinline__ uint32_t mx_quantize_quad(const float (&v)[8], uint32_t &scale) {
-    uint32_t top = 0;  // of the magnitudes' bits, so that an infinity or a NaN is the largest
+    float amax = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    const uint32_t field = top >> 23;
+    for (int i = 0; i < 8; ++i) amax = max_nan(amax, fabsf(v[i]));
+    amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+    amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+    const uint32_t field = __float_as_uint(amax) >> 23;  // 255: infinity or NaN
     scale = field == 255u ? 255u : field > 2u ? field - 2u : 0u;
     if (field == 255u) return 0u;
     const float inv = __uint_as_float((254u - scale) << 23);  // 2^-e
-    uint32_t codes = 0;
+    float r[8];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        uint32_t two;
-        asm("{\n"
-            ".reg .b8 t;\n"
-            "cvt.rn.satfinite.e2m1x2.f32 t, %2, %1;\n"
-            "cvt.u32.u8 %0, t;\n"
-            "}\n"
-            : "=r"(two)
-            : "f"(__fmul_rn(v[2 * i], inv)), "f"(__fmul_rn(v[2 * i + 1], inv)));
-        codes |= two << (8 * i);
-    }
+    for (int i = 0; i < 8; ++i) r[i] = __fmul_rn(v[i], inv);
+    uint32_t codes;
+    asm("{\n"
+        ".reg .b8 a, b, c, d;\n"
+        "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n"
+        "cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n"
+        "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n"
+        "cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n"
+        "mov.b32 %0, {a, b, c, d};\n"
+        "}\n"
+        : "=r"(codes)
+        : "f"(r[0]), "f"(r[1]), "f"(r[2]), "f"(r[3]), "f"(r[4]), "f"(r[5]), "f"(r[6]), "f"(r[7]));
     return codes;
 }
 
-// One warp per (row, unit): 256 elements to 128 bytes of codes and eight scales of the image of tiles of T rows.  Rows from m to
-// the end of the last tile and elements past k are zeros.  trigger: the stream's next kernel may start; not behind a kernel that
-// writes weights, which later kernels read without waiting.
-__global__ void __launch_bounds__(256) mx_quantize_kernel(const void *__restrict__ x, int x_type, int64_t m, int k, int units, int T, int64_t rows,
-                                                          uint8_t *__restrict__ image, int trigger) {
-    if (trigger) launch_dependents();
-    wait_predecessor();
-    const int lane = threadIdx.x & 31;
-    const int64_t item = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
-    const int64_t row = item / units;
-    const int u = (int)(item - row * units);
-    if (row >= rows) return;  // whole warp
-    const int e = u * kMxUnit + lane * 8;
-    float v[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = 0.0f;
-    if (row < m && e < k) load8(x, x_type, row * k + e, v);
+// Codes (128 bytes) and scales of one unit of row r of a tile, by a warp with elements 8 lane .. 8 lane + 7 in v.
+__device__ __forceinline__ void mx_store_unit(const float (&v)[8], uint8_t *unit, int T, int parts, int r, int lane) {
     uint32_t scale;
     const uint32_t codes = mx_quantize_quad(v, scale);
-    const int64_t tile = row / T;
-    const int r = (int)(row - tile * T);
-    uint8_t *unit = image + (tile * units + u) * mx_unit_bytes(T);
-    *reinterpret_cast<uint32_t *>(unit + mx_chunk_offset(r, lane >> 2) + (lane & 3) * 4) = codes;
-    // the scales of four blocks make a word: lanes 0, 4, 8, 12 and 16, 20, 24, 28
-    uint32_t word = 0;
+    const int rows = parts == 2 ? T / 2 : T, part = parts == 2 && r >= rows ? 1 : 0, part_bytes = rows * 128 + mx_scale_bytes(T);
+    *reinterpret_cast<uint32_t *>(unit + part * part_bytes + mx_chunk_offset(r - part * rows, lane >> 2) + (lane & 3) * 4) = codes;
+    if ((lane & 3) == 0) {
+        uint8_t *at = unit + mx_scale_offset(rows, r, lane >> 2);
+        *at = (uint8_t)scale;
+        if (parts == 2) at[part_bytes] = (uint8_t)scale;
+    }
+}
+
+// Rows of x to the image of tiles of T rows: a warp has two units of a row, `across` warps of a CTA lie along it.  Rows from m to the
+// end of the last tile and elements past k are zeros.  trigger: the stream's next kernel may start; not behind a kernel that writes weights,
+// which later kernels read without waiting.
+constexpr int kQuantUnits = 2;
+template <int X_TYPE>
+__global__ void __launch_bounds__(256) mx_quantize_kernel(const void *__restrict__ x, int m, int k, int units, int T, int parts, int rows,
+                                                          int across, uint8_t *__restrict__ image, int trigger) {
+    if (trigger) launch_dependents();
+    wait_predecessor();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int row = (int)blockIdx.x * (8 / across) + warp / across, u0 = ((int)blockIdx.y * across + warp % across) * kQuantUnits;
+    if (row >= rows || u0 >= units) return;  // whole warp
+    const int64_t from = (int64_t)row * k + u0 * kMxUnit + lane * 8;
+    const int left = row < m ? k - (u0 * kMxUnit + lane * 8) : 0;  // elements of the row from there
+    float v[kQuantUnits][8];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) word |= __shfl_sync(0xffffffffu, scale, (lane & 16) + 4 * i) << (8 * i);
-    if ((lane & 15) == 0) *reinterpret_cast<uint32_t *>(unit + mx_scale_offset(T, r, lane >> 2)) = word;
+    for (int j = 0; j < kQuantUnits; ++j) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[j][i] = 0.0f;
+        if (j * kMxUnit < left) load8(x, X_TYPE, from + j * kMxUnit, v[j]);
+    }
+    const int tile = row / T;
+    uint8_t *unit = image + ((int64_t)tile * units + u0) * mx_unit_bytes(T, parts);
+#pragma unroll
+    for (int j = 0; j < kQuantUnits; ++j)
+        if (u0 + j < units) mx_store_unit(v[j], unit + (int64_t)j * mx_unit_bytes(T, parts), T, parts, row - tile * T, lane);
 }
 
 // A file's 17-byte blocks (scale, then elements 0..15 in the low and 16..31 in the high halves of 16 bytes) to the weight image,
@@ -221,42 +240,60 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&v)[16]) {
 }
 
 constexpr int kMxMaxStages = 12;
-constexpr int kMxThreads = 192;  // warps 0-3 epilogue, 4 copies, 5 MMA
+constexpr int kMxQuantWarps = 8;              // quantize in the prologue; the first four are the epilogue
+constexpr int kMxThreads = 32 * (kMxQuantWarps + 2);  // and one warp copies, one issues MMAs
 
 struct MxParams {
     const uint8_t *w, *a;  // images: weights (tiles of 128 rows), activations (tiles of bn rows)
+    const void *x;         // or the activations themselves, which this kernel quantizes (a tile of 16 rows)
+    int x_type;
     void *y;
     int y_type;
     int64_t ldy;
-    int m, n, units;
+    int m, n, k, units;
     int bn, m_tiles;       // activation rows per tile (a multiple of 16, at most 256: the MMA's N)
     int split;             // CTAs of a cluster, which share the units of a tile
     int stages, stage_bytes;
+    int resident;          // bytes in front of the stages: the CTA's part of K of all activations, where it quantizes them
     int tmem_cols;
+    int wide;              // four outputs of a row may be stored together
 };
 
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
-__device__ __forceinline__ float ld_cluster(uint32_t smem, int rank) {
-    float v;
+__device__ __forceinline__ float4 ld_cluster4(uint32_t smem, int rank) {
+    float4 v;
     asm volatile(
         "{\n\t"
         ".reg .b32 r;\n\t"
-        "mapa.shared::cluster.u32 r, %1, %2;\n\t"
-        "ld.shared::cluster.f32 %0, [r];\n\t"
+        "mapa.shared::cluster.u32 r, %4, %5;\n\t"
+        "ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [r];\n\t"
         "}\n"
-        : "=f"(v)
+        : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
         : "r"(smem), "r"(rank)
         : "memory");
     return v;
 }
+__device__ __forceinline__ void put4(float *y, const float4 &v) { *reinterpret_cast<float4 *>(y) = v; }
+__device__ __forceinline__ void put4(__half *y, const float4 &v) {
+    const __half2 a = __floats2half2_rn(v.x, v.y), b = __floats2half2_rn(v.z, v.w);
+    *reinterpret_cast<uint2 *>(y) = make_uint2(*reinterpret_cast<const uint32_t *>(&a), *reinterpret_cast<const uint32_t *>(&b));
+}
+__device__ __forceinline__ void put4(__nv_bfloat16 *y, const float4 &v) {
+    const __nv_bfloat162 a = __floats2bfloat162_rn(v.x, v.y), b = __floats2bfloat162_rn(v.z, v.w);
+    *reinterpret_cast<uint2 *>(y) = make_uint2(*reinterpret_cast<const uint32_t *>(&a), *reinterpret_cast<const uint32_t *>(&b));
+}
 
 // One 128 x bn tile per cluster; its CTAs take equal parts of K, and the parts' sums meet in shared memory in a fixed order.
+// QUANTIZE: up to sixteen activation rows, which every CTA quantizes itself, its part of K, while the first weights are on their way: one launch
+// instead of two.
 // Ends in every case: waits are bounded, and a CTA that gave up still meets the others.
+template <bool QUANTIZE>
 __global__ void __launch_bounds__(kMxThreads, 1) mx_gemm_kernel(const __grid_constant__ MxParams p) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    uint64_t *full = reinterpret_cast<uint64_t *>(smem + p.stages * p.stage_bytes), *empty = full + kMxMaxStages, *done = empty + kMxMaxStages;
+    uint8_t *ring = smem + (QUANTIZE ? p.resident : 0);
+    uint64_t *full = reinterpret_cast<uint64_t *>(ring + p.stages * p.stage_bytes), *empty = full + kMxMaxStages, *done = empty + kMxMaxStages;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(done + 1);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
 
@@ -265,8 +302,8 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx_gemm_kernel(const __grid_con
     const int mt = tile % p.m_tiles, nt = tile / p.m_tiles;
     const int u0 = (int)((int64_t)p.units * rank / p.split), u1 = (int)((int64_t)p.units * (rank + 1) / p.split);
     const int count = u1 - u0;
-    constexpr int kABytes = mx_unit_bytes(kMxTile);
-    const int b_bytes = mx_unit_bytes(p.bn);
+    constexpr int kABytes = mx_unit_bytes(kMxTile), kQuantUnit = mx_unit_bytes(16);
+    const int b_bytes = QUANTIZE ? 0 : mx_unit_bytes(p.bn);
 
     launch_dependents();
     if (threadIdx.x == 0) {
@@ -279,24 +316,25 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx_gemm_kernel(const __grid_con
         fence_mbar_init();
     }
     __syncthreads();
-    if (warp == 4) {
+    if (warp == kMxQuantWarps) {
         // ---- operand tiles ----
         if (lane == 0) {
             const uint8_t *w = p.w + ((int64_t)nt * p.units + u0) * kABytes, *a = p.a + ((int64_t)mt * p.units + u0) * b_bytes;
             const int first = count < p.stages ? count : p.stages;
             for (int i = 0; i < first; ++i) {
                 mbar_arrive_expect_tx(&full[i], (uint32_t)(kABytes + b_bytes));
-                bulk_g2s(smem + i * p.stage_bytes, w + (int64_t)i * kABytes, kABytes, &full[i]);
+                bulk_g2s(ring + i * p.stage_bytes, w + (int64_t)i * kABytes, kABytes, &full[i]);
             }
             wait_predecessor();  // the activation image is there
-            for (int i = 0; i < first; ++i) bulk_g2s(smem + i * p.stage_bytes + kABytes, a + (int64_t)i * b_bytes, (uint32_t)b_bytes, &full[i]);
+            if (!QUANTIZE)
+                for (int i = 0; i < first; ++i) bulk_g2s(ring + i * p.stage_bytes + kABytes, a + (int64_t)i * b_bytes, (uint32_t)b_bytes, &full[i]);
             int s = 0;
             uint32_t par = 0;
             for (int i = first; i < count; ++i) {
-                if (!mbar_wait_abortable<32>(&empty[s], par, abort_flag)) break;
+                if (!mbar_wait_abortable<0>(&empty[s], par, abort_flag)) break;
                 mbar_arrive_expect_tx(&full[s], (uint32_t)(kABytes + b_bytes));
-                bulk_g2s(smem + s * p.stage_bytes, w + (int64_t)i * kABytes, kABytes, &full[s]);
-                bulk_g2s(smem + s * p.stage_bytes + kABytes, a + (int64_t)i * b_bytes, (uint32_t)b_bytes, &full[s]);
+                bulk_g2s(ring + s * p.stage_bytes, w + (int64_t)i * kABytes, kABytes, &full[s]);
+                if (!QUANTIZE) bulk_g2s(ring + s * p.stage_bytes + kABytes, a + (int64_t)i * b_bytes, (uint32_t)b_bytes, &full[s]);
                 if (++s == p.stages) {
                     s = 0;
                     par ^= 1;
@@ -304,21 +342,21 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx_gemm_kernel(const __grid_con
             }
         }
         __syncwarp();
-    } else if (warp == 5) {
+    } else if (warp == kMxQuantWarps + 1) {
         // ---- MMA ----
         // Tensor memory is taken only once the kernel before has finished: one that has yet to take all of it may still be starting.
         wait_predecessor();
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"((uint32_t)p.tmem_cols)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-        asm volatile("bar.sync 1, 160;" ::: "memory");  // with the epilogue warps
+        asm volatile("bar.sync 1, %0;" ::"n"(32 * (kMxQuantWarps + 1)) : "memory");  // with the quantizing and the epilogue warps
         const uint32_t tmem = *tmem_slot;
         if (elect_one()) {
             const uint32_t sfa = tmem + (uint32_t)((p.bn + 31) / 32 * 32), sfb = sfa + 8;
             const int groups = (p.bn + 127) / 128;
             // E2M1 both, E8M0 scales, K-major both, N, M = 128
             const uint32_t idesc = (1u << 7) | (1u << 10) | ((uint32_t)(p.bn >> 3) << 17) | (1u << 23) | (1u << 27);
-            const uint32_t base = smem_u32(smem);
+            const uint32_t base = smem_u32(ring);
             bool ok = true;
             int s = 0;
             uint32_t par = 0;
@@ -326,19 +364,19 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx_gemm_kernel(const __grid_con
                 ok = mbar_wait_abortable<0>(&full[s], par, abort_flag);
                 if (!ok) break;
                 tc_fence_after();
-                const uint32_t at = base + (uint32_t)(s * p.stage_bytes), bt = at + kABytes;
+                const uint32_t at = base + (uint32_t)(s * p.stage_bytes), bt = QUANTIZE ? smem_u32(smem) + (uint32_t)(i * kQuantUnit) : at + kABytes;
                 const uint32_t sa = umma_desc_lo(at + kMxTile * 128, 128), sb = umma_desc_lo(bt + (uint32_t)p.bn * 128, 128);
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     copy_scales(sfa + 4 * j, sa + j * (512 >> 4));
-                    for (int g = 0; g < groups; ++g) copy_scales(sfb + (uint32_t)(j * 4 * groups + 4 * g), sb + (uint32_t)((g * 1024 + j * 512) >> 4));
+                    copy_scales(sfb + 8 * j, sb + j * (512 >> 4));
+                    if (!QUANTIZE && groups == 2) copy_scales(sfb + 8 * j + 4, sb + (1024 >> 4) + j * (512 >> 4));
                 }
                 const uint32_t a_lo = umma_desc_lo(at, 16), b_lo = umma_desc_lo(bt, 16);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {  // 64 elements: 32 bytes along the swizzled rows
                     const uint32_t ids = (j & 1) ? (2u << 4) | (2u << 29) : 0u;
-                    umma_mxf4(tmem, a_lo + 2 * j, b_lo + 2 * j, idesc | ids, sfa + 4 * (j >> 1), sfb + (uint32_t)((j >> 1) * 4 * groups),
-                              i > 0 || j > 0 ? 1u : 0u);
+                    umma_mxf4(tmem, a_lo + 2 * j, b_lo + 2 * j, idesc | ids, sfa + 4 * (j >> 1), sfb + 8 * (j >> 1), i > 0 || j > 0 ? 1u : 0u);
                 }
                 umma_commit(&empty[s]);
                 if (++s == p.stages) {
@@ -349,47 +387,50 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx_gemm_kernel(const __grid_con
             umma_commit(done);
         }
         __syncwarp();
+    } else {
+        wait_predecessor();  // the time limit of the wait for the sums counts from here
+        if (QUANTIZE) {
+            // a warp takes (row, unit) after (row, unit), four at a time
+            const int items = p.m * count;
+            for (int i0 = warp; i0 < items; i0 += 4 * kMxQuantWarps) {
+                float v[4][8];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int i = i0 + j * kMxQuantWarps, r = i / count, e = (u0 + i - r * count) * kMxUnit + lane * 8;
+#pragma unroll
+                    for (int q = 0; q < 8; ++q) v[j][q] = 0.0f;
+                    if (i < items && e < p.k) load8(p.x, p.x_type, (int64_t)r * p.k + e, v[j]);
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int i = i0 + j * kMxQuantWarps, r = i / count;
+                    if (i < items) mx_store_unit(v[j], smem + (i - r * count) * kQuantUnit, 16, 1, r, lane);
+                }
+            }
+            fence_proxy_async();  // the tensor cores read what was written here
+        }
+        asm volatile("bar.sync 1, %0;" ::"n"(32 * (kMxQuantWarps + 1)) : "memory");
     }
     // ---- epilogue ----
     if (warp < 4) {
-        wait_predecessor();  // the time limit of the wait below counts from here
-        asm volatile("bar.sync 1, 160;" ::: "memory");
         const bool ok = mbar_wait_abortable<64>(done, 0, abort_flag);
         tc_fence_after();
         const uint32_t tmem = *tmem_slot + ((uint32_t)(warp * 32) << 16);
-        const int r = warp * 32 + lane;
-        const int64_t n = (int64_t)nt * kMxTile + r;
-        if (!ok) {
-            // nothing to read or store
-        } else if (p.split == 1) {
-            for (int c0 = 0; c0 < p.bn; c0 += 16) {
-                uint32_t v[16];
-                tmem_ld16(tmem + (uint32_t)c0, v);
-                tmem_ld_wait();
-                loaded(v);
-                const int left = p.m - (mt * p.bn + c0);  // rows of x
-                if (n < p.n)
-                    with_y_type(p.y, p.y_type, [&](auto *y) {
-#pragma unroll
-                        for (int j = 0; j < 16; ++j)
-                            if (j < left) put_y(y, ((int64_t)mt * p.bn + c0 + j) * p.ldy + n, __uint_as_float(v[j]));
-                    });
-            }
-        } else {
-            float *part = reinterpret_cast<float *>(smem);  // [bn][128]; every copy and MMA has finished with the stages
+        if (ok) {
+            float *part = reinterpret_cast<float *>(smem);  // [bn][128]; every copy and MMA has finished with the memory
             for (int c0 = 0; c0 < p.bn; c0 += 16) {
                 uint32_t v[16];
                 tmem_ld16(tmem + (uint32_t)c0, v);
                 tmem_ld_wait();
                 loaded(v);
 #pragma unroll
-                for (int j = 0; j < 16; ++j) part[(c0 + j) * kMxTile + r] = __uint_as_float(v[j]);
+                for (int j = 0; j < 16; ++j) part[(c0 + j) * kMxTile + warp * 32 + lane] = __uint_as_float(v[j]);
             }
         }
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 5) {
+    if (warp == kMxQuantWarps + 1) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(*tmem_slot), "r"((uint32_t)p.tmem_cols));
     }
@@ -397,17 +438,37 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx_gemm_kernel(const __grid_con
         __syncwarp();
         cluster_arrive();
         cluster_wait();
+    }
+    {
         const int rows = min(p.bn, p.m - mt * p.bn);
         const int c0 = rows * rank / p.split, c1 = rows * (rank + 1) / p.split;
         const uint32_t part = smem_u32(smem);
+        const int64_t n = (int64_t)nt * kMxTile + 4 * lane;
         with_y_type(p.y, p.y_type, [&](auto *y) {
-            for (int i = c0 * kMxTile + threadIdx.x; i < c1 * kMxTile; i += kMxThreads) {
-                const int64_t n = (int64_t)nt * kMxTile + (i & (kMxTile - 1));
-                float sum = 0.0f;
-                for (int q = 0; q < p.split; ++q) sum += ld_cluster(part + 4u * (uint32_t)i, q);
-                if (n < p.n) put_y(y, ((int64_t)mt * p.bn + (i >> 7)) * p.ldy + n, sum);
+            // a warp per row of outputs, four per lane (straight from tensor memory a store has 32: 14336 outputs of 128 rows took 3 us longer)
+            for (int c = c0 + warp; c < c1; c += kMxThreads / 32) {
+                float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 8
+                for (int q = 0; q < p.split; ++q) {
+                    const float4 v = ld_cluster4(part + 16u * (uint32_t)(c * (kMxTile / 4) + lane), q);
+                    sum.x += v.x;
+                    sum.y += v.y;
+                    sum.z += v.z;
+                    sum.w += v.w;
+                }
+                auto *out = y + ((int64_t)mt * p.bn + c) * p.ldy + n;
+                if (p.wide && n + 4 <= p.n) {
+                    put4(out, sum);
+                } else {
+                    if (n < p.n) put_y(out, 0, sum.x);
+                    if (n + 1 < p.n) put_y(out, 1, sum.y);
+                    if (n + 2 < p.n) put_y(out, 2, sum.z);
+                    if (n + 3 < p.n) put_y(out, 3, sum.w);
+                }
             }
         });
+    }
+    if (p.split > 1) {
         cluster_arrive();
         cluster_wait();  // the others may still read this CTA's part
     }
@@ -422,12 +483,12 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx_gemm_kernel(const __grid_con
 // may only signal their own CTA, and passing that on by a thread (wait, arrive across the cluster) cost a microsecond a stage, four times
 // the stage's work.  The maps see an image as rows of 128 bytes.
 constexpr int kPairMaxBn = 240;  // two accumulators and the scales fill the 512 columns
-constexpr int kPairStages = 6;
+constexpr int kPairStages = 12;
 constexpr int kPairEpiWarps = 8;
 constexpr int kPairThreads = 32 * (kPairEpiWarps + 2);
 
 struct MxPairParams {
-    CUtensorMap w, codes, scales;  // boxes of a unit's rows of 128 bytes: of weights; of half of the activations' codes; of their scales
+    CUtensorMap w, a;  // boxes of a unit's rows of 128 bytes: of weights; of one part of the activations
     void *y;
     int y_type;
     int64_t ldy;
@@ -494,7 +555,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) mx_gemm_pair_kernel(const __g
     const int rank = blockIdx.x & 1;
     const int tiles = (p.n_tiles + 1) / 2 * p.m_tiles, first = blockIdx.x >> 1, step = gridDim.x >> 1;
     constexpr int kABytes = mx_unit_bytes(kMxTile);
-    const int half = p.bn / 2 * 128, scales = mx_scale_bytes(p.bn), unit_rows = p.bn + scales / 128;
+    const int half = p.bn / 2 * 128, part_bytes = half + mx_scale_bytes(p.bn), part_rows = part_bytes / 128;
 
     launch_dependents();
     if (threadIdx.x == 0) {
@@ -531,7 +592,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) mx_gemm_pair_kernel(const __g
             const uint32_t full0 = mapa(smem_u32(full), 0);
             for (int t = first; t < tiles && ok; t += step) {
                 const int mt = t % p.m_tiles, nt = min(t / p.m_tiles * 2 + rank, p.n_tiles - 1);  // an odd last tile: once more, not stored
-                int w = nt * p.units * (kABytes / 128), a = mt * p.units * unit_rows;  // rows of 128 bytes
+                int w = nt * p.units * (kABytes / 128), a = (mt * p.units * 2 + rank) * part_rows;  // rows of 128 bytes
                 for (int u = 0; u < p.units; ++u) {
                     if (fill >= p.stages) {
                         ok = mbar_wait_abortable<0>(&empty[s], par, abort_flag);
@@ -541,12 +602,11 @@ __global__ void __launch_bounds__(kPairThreads, 1) mx_gemm_pair_kernel(const __g
                     }
                     uint8_t *dst = smem + s * p.stage_bytes;
                     const uint32_t bar = full0 + 8u * (uint32_t)s;
-                    if (rank == 0) mbar_arrive_expect_tx(&full[s], (uint32_t)(2 * (kABytes + half + scales)));
+                    if (rank == 0) mbar_arrive_expect_tx(&full[s], (uint32_t)(2 * (kABytes + part_bytes)));
                     copy_rows(dst, &p.w, w, bar);
-                    copy_rows(dst + kABytes, &p.codes, a + rank * (p.bn / 2), bar);
-                    copy_rows(dst + kABytes + half, &p.scales, a + p.bn, bar);
+                    copy_rows(dst + kABytes, &p.a, a, bar);
                     w += kABytes / 128;
-                    a += unit_rows;
+                    a += 2 * part_rows;
                     if (++s == p.stages) {
                         s = 0;
                         par ^= 1;
@@ -621,12 +681,15 @@ __global__ void __launch_bounds__(kPairThreads, 1) mx_gemm_pair_kernel(const __g
                     tmem_ld16(from + (uint32_t)c, v);
                     tmem_ld_wait();
                     loaded(v);
-                    const int row = mt * p.bn + c, left = p.m - row;
+                    const int row = mt * p.bn + c, left = n < p.n ? p.m - row : 0;
                     auto *at = y + (int64_t)row * p.ldy + n;
-                    if (n < p.n) {
+                    if (left >= 16) {
 #pragma unroll
-                        for (int j = 0; j < 16; ++j)
-                            if (j < left) put_y(at + (int64_t)j * p.ldy, 0, __uint_as_float(v[j]));
+                        for (int j = 0; j < 16; ++j, at += p.ldy) put_y(at, 0, __uint_as_float(v[j]));
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 16; ++j, at += p.ldy)
+                            if (j < left) put_y(at, 0, __uint_as_float(v[j]));
                     }
                 }
             });
@@ -664,14 +727,21 @@ int mx_check(int64_t m, int64_t n, int64_t k) {
     return LLOOM_OK;
 }
 
-int64_t mx_image_bytes(int64_t rows, int64_t k, int T) { return (rows + T - 1) / T * mx_units(k) * mx_unit_bytes(T); }
+int64_t mx_image_bytes(int64_t rows, int64_t k, int T, int parts = 1) { return (rows + T - 1) / T * mx_units(k) * mx_unit_bytes(T, parts); }
 
-int launch_mx_quantize(const void *x, int x_type, int64_t m, int64_t k, int T, uint8_t *image, bool trigger, bool overlap,
+int launch_mx_quantize(const void *x, int x_type, int64_t m, int64_t k, int T, int parts, uint8_t *image, bool trigger, bool overlap,
                        cudaStream_t stream) {
-    const int64_t rows = (m + T - 1) / T * T, grid = ceil_div64(rows * mx_units(k), 8);
-    if (grid > 0x7fffffff) return LLOOM_ERR_SHAPE;
-    return launch_status(launch_early(mx_quantize_kernel, (unsigned)grid, 256, 0, overlap, stream, x, x_type, m, (int)k, (int)mx_units(k), T, rows,
-                                      image, trigger ? 1 : 0));
+    const int64_t rows = (m + T - 1) / T * T, units = mx_units(k);
+    if (rows > 0x7fffffff) return LLOOM_ERR_SHAPE;
+    int across = 1;
+    while (across < 8 && across * kQuantUnits < units) across *= 2;
+    const dim3 grid((unsigned)ceil_div64(rows, 8 / across), (unsigned)ceil_div64(units, kQuantUnits * across));
+    if (grid.y > 65535) return LLOOM_ERR_SHAPE;
+    auto kern = x_type == LLOOM_F32   ? mx_quantize_kernel<LLOOM_F32>
+                : x_type == LLOOM_F16 ? mx_quantize_kernel<LLOOM_F16>
+                                      : mx_quantize_kernel<LLOOM_BF16>;
+    return launch_status(launch_early(kern, grid, 256, 0, overlap, stream, x, (int)m, (int)k, (int)units, T, parts, (int)rows, across, image,
+                                      trigger ? 1 : 0));
 }
 
 // Tiles for pairs of CTAs: of the widths that fit, the one with the least time over the rounds that the pairs make, a unit of K taking
@@ -694,19 +764,27 @@ MxTiles mx_pair_tiles(int64_t m, int64_t n, int pairs) {
 }
 
 struct MxPlan {
-    bool pairs;
+    bool pairs, quantize;
     MxTiles tiles;
+    int split;
 };
 MxPlan mx_plan(int64_t m, int64_t n, int64_t k, int sms) {
     MxPlan pl;
-    pl.pairs = m > 128;
-    pl.tiles = pl.pairs ? mx_pair_tiles(m, n, sms / 2) : mx_tiles(m, (m + 255) / 256);
+    const int64_t units = mx_units(k);
+    pl.tiles = mx_pair_tiles(m, n, sms / 2);
+    const int64_t pair_tiles = (n + 2 * kMxTile - 1) / (2 * kMxTile) * pl.tiles.count;
+    pl.pairs = m > 128 && (units <= 32 || pair_tiles * 4 >= sms);
+    if (!pl.pairs) pl.tiles = mx_tiles(m, (m + 255) / 256);
+    const int64_t tiles = (n + kMxTile - 1) / kMxTile * pl.tiles.count;
+    for (pl.split = 1; pl.split < 8 && tiles * pl.split * 2 <= sms && units >= pl.split * 2; pl.split *= 2) {}
+    const int64_t part = (units + pl.split - 1) / pl.split;
+    pl.quantize = m <= 16 && m * part <= 32;
     return pl;
 }
 // Bytes of the activation image, whatever the device's plan: the largest of all tile widths
 int64_t mx_act_bytes(int64_t m, int64_t k) {
     int64_t most = 0;
-    for (int T = 16; T <= 256; T += 16) most = std::max(most, (m + T - 1) / T * mx_unit_bytes(T));
+    for (int T = 16; T <= 256; T += 16) most = std::max(most, (m + T - 1) / T * mx_unit_bytes(T, 2));
     return most * mx_units(k);
 }
 
@@ -716,11 +794,11 @@ struct MxSmemOnce {
 };
 
 template <class Params>
-int launch_mx_gemm(void (*kern)(Params), MxSmemOnce &once, const Params &p, int ctas, int cluster, int threads, cudaStream_t stream) {
+int launch_mx_gemm(void (*kern)(Params), MxSmemOnce &once, const Params &p, int stages, int ctas, int cluster, int threads, bool early, cudaStream_t stream) {
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess || dev < 0 || dev >= 64) return LLOOM_ERR_DEVICE;
-    const int smem = p.stages * p.stage_bytes + 256 + 1024;
+    const int smem = stages + 256 + 1024;
     {
         std::lock_guard<std::mutex> lock(once.mu);
         if (!once.done[dev]) {
@@ -735,14 +813,14 @@ int launch_mx_gemm(void (*kern)(Params), MxSmemOnce &once, const Params &p, int 
     cfg.dynamicSmemBytes = (size_t)smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = (unsigned)cluster;
-    attr[1].val.clusterDim.y = 1;
-    attr[1].val.clusterDim.z = 1;
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)cluster;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 2;
+    cfg.numAttrs = early ? 2 : 1;
     return launch_status(cudaLaunchKernelEx(&cfg, kern, p));
 }
 
@@ -762,18 +840,21 @@ int mx_forward(const void *image, const void *x, int x_type, void *y, int y_type
     if (rc != LLOOM_OK) return rc;
     const MxPlan pl = mx_plan(m, n, k, di.sm_count);
     const MxTiles t = pl.tiles;
-    // The product starts on the weights while this kernel runs, so it is not launched early itself unless they are in place.
-    rc = launch_mx_quantize(x, x_type, m, k, t.bn, (uint8_t *)workspace, true, overlap, (cudaStream_t)stream);
-    if (rc != LLOOM_OK) return rc;
+    // The product may start while the quantizer runs; the quantizer itself (or the product that does its work) starts under the kernel in front
+    // only if the weights are in place.
+    if (!pl.quantize) {
+        rc = launch_mx_quantize(x, x_type, m, k, t.bn, pl.pairs ? 2 : 1, (uint8_t *)workspace, true, overlap, (cudaStream_t)stream);
+        if (rc != LLOOM_OK) return rc;
+    }
     const int64_t n_tiles = (n + kMxTile - 1) / kMxTile;
     const int units = (int)mx_units(k);
     if (pl.pairs) {
         static MxSmemOnce once;
         MxPairParams p = {};
-        const int64_t w_rows = mx_image_bytes(n, k, kMxTile) / 128, a_rows = mx_image_bytes(m, k, t.bn) / 128;
+        const int64_t w_rows = mx_image_bytes(n, k, kMxTile) / 128, a_rows = mx_image_bytes(m, k, t.bn, 2) / 128;
         if (w_rows > 0x7fffffff || a_rows > 0x7fffffff) return LLOOM_ERR_SHAPE;  // 256 GB
-        if (!encode_rows_map(p.w, image, w_rows, 128, 128, mx_unit_bytes(kMxTile) / 128) || !encode_rows_map(p.codes, workspace, a_rows, 128, 128, t.bn / 2) ||
-            !encode_rows_map(p.scales, workspace, a_rows, 128, 128, mx_scale_bytes(t.bn) / 128))
+        if (!encode_rows_map(p.w, image, w_rows, 128, 128, mx_unit_bytes(kMxTile) / 128) ||
+            !encode_rows_map(p.a, workspace, a_rows, 128, 128, mx_unit_bytes(t.bn, 2) / 256))
             return LLOOM_ERR_DEVICE;
         p.y = y;
         p.y_type = y_type;
@@ -790,30 +871,36 @@ int mx_forward(const void *image, const void *x, int x_type, void *y, int y_type
         const int64_t tiles = (n_tiles + 1) / 2 * t.count;
         if (tiles > 0x3fffffff) return LLOOM_ERR_SHAPE;
         const int pairs = (int)(tiles < di.sm_count / 2 ? tiles : di.sm_count / 2);
-        return launch_mx_gemm(mx_gemm_pair_kernel, once, p, 2 * pairs, 2, kPairThreads, (cudaStream_t)stream);
+        return launch_mx_gemm(mx_gemm_pair_kernel, once, p, p.stages * p.stage_bytes, 2 * pairs, 2, kPairThreads, true, (cudaStream_t)stream);
     }
-    static MxSmemOnce once;
+    static MxSmemOnce once, once_quantize;
     MxParams p = {};
     p.w = (const uint8_t *)image;
     p.a = (const uint8_t *)workspace;
+    p.x = x;
+    p.x_type = x_type;
     p.y = y;
     p.y_type = y_type;
     p.ldy = ldy;
     p.m = (int)m;
     p.n = (int)n;
+    p.k = (int)k;
     p.units = units;
     p.bn = t.bn;
     p.m_tiles = t.count;
-    const int64_t tiles = n_tiles * t.count;
-    p.split = 1;
-    while (p.split < 8 && tiles * p.split * 2 <= di.sm_count && p.units >= p.split * 2) p.split *= 2;
-    if (tiles * p.split > 0x7fffffff) return LLOOM_ERR_SHAPE;
-    p.stage_bytes = mx_unit_bytes(kMxTile) + mx_unit_bytes(t.bn);
-    p.stages = (di.max_smem_optin - 256 - 1024) / p.stage_bytes;
+    p.split = pl.split;
+    p.wide = ldy % 4 == 0 && aligned(y, 4 * elem_bytes(y_type));
+    const int64_t ctas = n_tiles * t.count * p.split;
+    if (ctas > 0x7fffffff) return LLOOM_ERR_SHAPE;
+    p.resident = pl.quantize ? (units + p.split - 1) / p.split * mx_unit_bytes(16) : 0;
+    p.stage_bytes = mx_unit_bytes(kMxTile) + (pl.quantize ? 0 : mx_unit_bytes(t.bn));
+    p.stages = (di.max_smem_optin - 256 - 1024 - p.resident) / p.stage_bytes;
     if (p.stages > kMxMaxStages) p.stages = kMxMaxStages;
-    const int cols = (t.bn + 31) / 32 * 32 + 8 + 8 * ((t.bn + 127) / 128);
+    const int cols = (t.bn + 31) / 32 * 32 + 24;
     for (p.tmem_cols = 32; p.tmem_cols < cols; p.tmem_cols *= 2) {}
-    return launch_mx_gemm(mx_gemm_kernel, once, p, (int)(tiles * p.split), p.split, kMxThreads, (cudaStream_t)stream);
+    const int smem = p.resident + p.stages * p.stage_bytes;
+    return pl.quantize ? launch_mx_gemm(mx_gemm_kernel<true>, once_quantize, p, smem, (int)ctas, p.split, kMxThreads, overlap, (cudaStream_t)stream)
+                       : launch_mx_gemm(mx_gemm_kernel<false>, once, p, smem, (int)ctas, p.split, kMxThreads, true, (cudaStream_t)stream);
 }
 
 int mx_quantize(const void *x, int x_type, int64_t rows, int64_t k, void *image, int64_t image_bytes, void *stream, bool overlap) {
@@ -823,7 +910,7 @@ int mx_quantize(const void *x, int x_type, int64_t rows, int64_t k, void *image,
     if (!x || !image) return LLOOM_ERR_NULL;
     if (image_bytes < mx_image_bytes(rows, k, kMxTile)) return LLOOM_ERR_WORKSPACE;
     if (!aligned(x, 16) || !aligned(image, 256)) return LLOOM_ERR_ALIGN;
-    return launch_mx_quantize(x, x_type, rows, k, kMxTile, (uint8_t *)image, false, overlap, (cudaStream_t)stream);
+    return launch_mx_quantize(x, x_type, rows, k, kMxTile, 1, (uint8_t *)image, false, overlap, (cudaStream_t)stream);
 }
 
 int mx_dequantize(const void *image, int64_t rows, int64_t k, void *out, bool f16, void *stream, bool overlap) {

@@ -23,30 +23,24 @@ namespace {
 struct NormParams {
     const void *x, *r, *w;  // r may be null
     void *h, *y;            // h: null exactly when r is
-    int x_type, w_type, y_type;  // y_type: x_type's own, LLOOM_Q8_0 or LLOOM_Q8_K
-    int vec;                // rows and weights start on 16 bytes and k is a multiple of 8
+    int w_type, y_type;     // y_type: x's own, LLOOM_Q8_0 or LLOOM_Q8_K
+    int lanes;              // threads on a row where they are fewer than a warp's, else 0: the CTA's threads
     int64_t m, ldx, ldr;
     int k;
-    double eps;
+    double per_k, eps;  // per_k: 1 / k
 };
 
-// elements e .. e + 7 of a row, zeros past its end
-__device__ __forceinline__ void load_octet(const void *p, int type, int64_t row, int e, int k, int vec, float (&v)[8]) {
-    if (vec) {
-        load8(p, type, row + e, v);
-        return;
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        v[i] = 0.0f;
-        if (e + i >= k) continue;
-        const int64_t at = row + e + i;
-        if (type == LLOOM_F32) v[i] = __ldg(reinterpret_cast<const float *>(p) + at);
-        else if (type == LLOOM_F16) v[i] = __half2float(__ldg(reinterpret_cast<const __half *>(p) + at));
-        else v[i] = __bfloat162float(__ldg(reinterpret_cast<const __nv_bfloat16 *>(p) + at));
-    }
+__device__ __forceinline__ float load_one(const void *p, int type, int64_t i) {
+    if (type == LLOOM_F32) return __ldg(reinterpret_cast<const float *>(p) + i);
+    if (type == LLOOM_F16) return __half2float(__ldg(reinterpret_cast<const __half *>(p) + i));
+    return __bfloat162float(__ldg(reinterpret_cast<const __nv_bfloat16 *>(p) + i));
 }
-
+// How the pieces of a row lie
+enum Pieces {
+    kAnywhere,  // element by element
+    kEdges,     // on 16-byte boundaries, the first and the last one partly outside of the row
+    kWhole      // on 16-byte boundaries, all of them inside
+};
 __device__ __forceinline__ uint32_t pack_halves(int type, float a, float b) {
     if (type == LLOOM_F16) {
         const __half2 h = __floats2half2_rn(a, b);
@@ -56,45 +50,123 @@ __device__ __forceinline__ uint32_t pack_halves(int type, float a, float b) {
     return *reinterpret_cast<const uint32_t *>(&h);
 }
 
-__device__ __forceinline__ void store_octet(void *p, int type, int64_t row, int e, int k, int vec, const float (&v)[8]) {
-    if (!vec) {
-        for (int i = 0; i < 8 && e + i < k; ++i) store_y(p, type, row + e + i, v[i]);
-    } else if (type == LLOOM_F32) {
-        float4 *q = reinterpret_cast<float4 *>(reinterpret_cast<float *>(p) + row + e);
-        q[0] = make_float4(v[0], v[1], v[2], v[3]);
-        q[1] = make_float4(v[4], v[5], v[6], v[7]);
-    } else {
-        *reinterpret_cast<uint4 *>(reinterpret_cast<unsigned short *>(p) + row + e) =
-            make_uint4(pack_halves(type, v[0], v[1]), pack_halves(type, v[2], v[3]), pack_halves(type, v[4], v[5]), pack_halves(type, v[6], v[7]));
+// Elements e .. e + 7 of a row, as they lie in memory: halves in four registers, so that more rows are in flight
+template <int TYPE>
+struct Piece {
+    static constexpr int kWords = TYPE == LLOOM_F32 ? 8 : 4;
+    uint32_t w[kWords];
+    __device__ __forceinline__ void put(const float (&v)[8]) {
+        if constexpr (TYPE == LLOOM_F32) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) w[i] = __float_as_uint(v[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = pack_halves(TYPE, v[2 * i], v[2 * i + 1]);
+        }
     }
-}
+    __device__ __forceinline__ void get(float (&v)[8]) const {
+        if constexpr (TYPE == LLOOM_F32) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(w[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                v[2 * i] = TYPE == LLOOM_F16 ? f16_bits_to_f32(w[i] & 0xffffu) : __uint_as_float(w[i] << 16);
+                v[2 * i + 1] = TYPE == LLOOM_F16 ? f16_bits_to_f32(w[i] >> 16) : __uint_as_float(w[i] & 0xffff0000u);
+            }
+        }
+    }
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) w[i] = 0u;
+    }
+    // from and to the row that starts at element `row` of p; zeros outside of 0 .. k - 1
+    template <int PIECES>
+    __device__ __forceinline__ void load(const void *p, int64_t row, int e, int k) {
+        if (PIECES == kWhole || (PIECES == kEdges && e >= 0 && e + 8 <= k)) {
+            const uint4 *q = reinterpret_cast<const uint4 *>(reinterpret_cast<const uint8_t *>(p) + (row + e) * (kWords / 2));
+#pragma unroll
+            for (int i = 0; i < kWords / 4; ++i) {
+                const uint4 t = __ldg(q + i);
+                w[4 * i] = t.x;
+                w[4 * i + 1] = t.y;
+                w[4 * i + 2] = t.z;
+                w[4 * i + 3] = t.w;
+            }
+        } else {
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = e + i >= 0 && e + i < k ? load_one(p, TYPE, row + e + i) : 0.0f;
+            put(v);
+        }
+    }
+    template <int PIECES>
+    __device__ __forceinline__ void store(void *p, int64_t row, int e, int k) const {
+        if (PIECES == kWhole || (PIECES == kEdges && e >= 0 && e + 8 <= k)) {
+            uint4 *q = reinterpret_cast<uint4 *>(reinterpret_cast<uint8_t *>(p) + (row + e) * (kWords / 2));
+#pragma unroll
+            for (int i = 0; i < kWords / 4; ++i) q[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+        } else {
+            float v[8];
+            get(v);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (e + i >= 0 && e + i < k) store_y(p, TYPE, row + e + i, v[i]);
+        }
+    }
+};
 
-__device__ __forceinline__ float round_to(int type, float v) {
-    if (type == LLOOM_F16) return __half2float(__float2half_rn(v));
-    if (type == LLOOM_BF16) return __bfloat162float(__float2bfloat16_rn(v));
+template <int X_TYPE>
+__device__ __forceinline__ float round_to(float v) {
+    if (X_TYPE == LLOOM_F16) return __half2float(__float2half_rn(v));
+    if (X_TYPE == LLOOM_BF16) return __bfloat162float(__float2bfloat16_rn(v));
     return v;
 }
 
-// The stream's elements h of an octet; stored if there is a residual
-__device__ __forceinline__ void stream_octet(const NormParams &p, int64_t row, int e, float (&v)[8]) {
-    load_octet(p.x, p.x_type, row * p.ldx, e, p.k, p.vec, v);
-    if (!p.r) return;
-    float r[8];
-    load_octet(p.r, p.x_type, row * p.ldr, e, p.k, p.vec, r);
+// x becomes h = x + r, which is stored, where there is a residual; its squares are added
+template <int X_TYPE, int PIECES>
+__device__ __forceinline__ void stream_piece(const NormParams &p, int64_t row, int e, bool live, Piece<X_TYPE> &x, const Piece<X_TYPE> &r, double (&sum)[2]) {
+    float v[8];
+    x.get(v);
+    if (p.r && live) {
+        float u[8];
+        r.get(u);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = round_to(p.x_type, __fadd_rn(v[i], r[i]));
-    store_octet(p.h, p.x_type, row * p.k, e, p.k, p.vec, v);
+        for (int i = 0; i < 8; ++i) v[i] = round_to<X_TYPE>(__fadd_rn(v[i], u[i]));
+        x.put(v);
+        x.template store<PIECES>(p.h, row * p.k, e, p.k);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum[i & 1] = fma((double)v[i], (double)v[i], sum[i & 1]);
 }
 
-__device__ __forceinline__ void square_sum(const float (&v)[8], double &sum) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) sum = fma((double)v[i], (double)v[i], sum);
+// 1 / sqrt(a), rounded to f32: Newton's iteration in 64 bits from the 32-bit approximation (2^-21, then below 2^-41, then 2^-53) where that one
+// is in range.  A row waits for this between its loads and its output, and the square root and the division take three times as long.
+__device__ __forceinline__ float inverse_root(double a) {
+    if (!(a > 1e-30 && a < 1e30)) return (float)(1.0 / sqrt(a));
+    double y = (double)rsqrtf((float)a);
+    const double half = 0.5 * a;
+    y = y * fma(-half * y, y, 1.5);
+    y = y * fma(-half * y, y, 1.5);
+    return (float)y;
 }
 
-// y of an octet from h; all lanes of a warp, `live` says whose octet lies in the row
+// An octet of weights, which lie like the row only where that starts on a boundary
+template <int PIECES>
+__device__ __forceinline__ void weight_octet(const NormParams &p, int e, float (&w)[8]) {
+    if (PIECES == kWhole) {
+        load8(p.w, p.w_type, e, w);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = e + i >= 0 && e + i < p.k ? load_one(p.w, p.w_type, e + i) : 0.0f;
+    }
+}
+
+// y of an octet from h and w; all lanes of a warp, `live` says whose octet lies in a row
+template <int X_TYPE, int PIECES>
 __device__ __forceinline__ void output_octet(const NormParams &p, int64_t row, int e, bool live, float inv, float (&v)[8]) {
     float w[8];
-    if (live) load_octet(p.w, p.w_type, 0, e, p.k, p.vec, w);
+    if (live) weight_octet<PIECES>(p, e, w);
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = live ? __fmul_rn(__fmul_rn(v[i], inv), w[i]) : 0.0f;
     if (p.y_type == LLOOM_Q8_K) {  // a warp has a 256-element block
@@ -124,73 +196,110 @@ __device__ __forceinline__ void output_octet(const NormParams &p, int64_t row, i
         q[2] = (unsigned short)(hi & 0xffffu);
         q[3] = (unsigned short)(hi >> 16);
     } else if (live) {
-        store_octet(p.y, p.y_type, row * p.k, e, p.k, p.vec, v);
+        Piece<X_TYPE> y;
+        y.put(v);
+        y.template store<PIECES>(p.y, row * p.k, e, p.k);
     }
 }
 
-// blockDim.x threads on a row (whole warps; blockDim.y rows per CTA, more than one only where a warp has a row to itself).
 // OCTETS: eight-element pieces a thread keeps in registers; 0: any number, read again from h (or x) for the output.
-template <int OCTETS>
-__global__ void __launch_bounds__(1024) rms_norm_kernel(const __grid_constant__ NormParams p) {
+// PIECES: kEdges where the rows of x, r, h and y lie alike modulo 16 bytes, kWhole where they start there, k is a multiple of eight and the weights
+// start there too.
+template <int X_TYPE, int OCTETS, int PIECES>
+__global__ void __launch_bounds__(OCTETS == 2 && X_TYPE != LLOOM_F32 ? 512 : 1024, OCTETS == 1 ? 2 : OCTETS == 2 && X_TYPE != LLOOM_F32 ? 3 : 1) rms_norm_kernel(const __grid_constant__ NormParams p) {
     __shared__ double part[32];
     launch_dependents();
     wait_predecessor();  // everything read or written here may be the predecessor's
-    const int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
-    if (row >= p.m) return;  // whole warps, and only where no one waits for them
-    const int warp_e = (threadIdx.x & ~31) * 8, e0 = threadIdx.x * 8, step = blockDim.x * 8;
+    const int lanes = p.lanes ? p.lanes : (int)blockDim.x, t = p.lanes ? (int)threadIdx.x % p.lanes : (int)threadIdx.x;
+    const int64_t row = p.lanes ? (int64_t)blockIdx.x * (blockDim.x / p.lanes) + threadIdx.x / p.lanes : (int64_t)blockIdx.x;
+    const bool has_row = row < p.m;
+    // elements in front of the row that its first piece would reach into
+    constexpr int size = X_TYPE == LLOOM_F32 ? 4 : 2;
+    const int pad = PIECES == kEdges ? (int)((reinterpret_cast<uintptr_t>(p.x) + (uintptr_t)(row * p.ldx) * size) & 15) / size : 0;
+    const int e0 = t * 8 - pad, step = lanes * 8;
     constexpr int N = OCTETS > 0 ? OCTETS : 1;
-    float v[N][8];
-    double sum = 0.0;
+    Piece<X_TYPE> h[N];
+    double sums[2] = {0.0, 0.0};
     if constexpr (OCTETS > 0) {
+        Piece<X_TYPE> r[N];
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int e = e0 + i * step;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[i][j] = 0.0f;
-            if (e < p.k) stream_octet(p, row, e, v[i]);
+            if (has_row && e < p.k) {
+                h[i].template load<PIECES>(p.x, row * p.ldx, e, p.k);
+                if (p.r) r[i].template load<PIECES>(p.r, row * p.ldr, e, p.k);
+            } else {
+                h[i].zero();
+            }
         }
 #pragma unroll
-        for (int i = 0; i < N; ++i) square_sum(v[i], sum);
+        for (int i = 0; i < N; ++i) stream_piece<X_TYPE, PIECES>(p, row, e0 + i * step, has_row && e0 + i * step < p.k, h[i], r[i], sums);
     } else {
         for (int e = e0; e < p.k; e += step) {
-            stream_octet(p, row, e, v[0]);
-            square_sum(v[0], sum);
+            Piece<X_TYPE> r;
+            h[0].template load<PIECES>(p.x, row * p.ldx, e, p.k);
+            if (p.r) r.template load<PIECES>(p.r, row * p.ldr, e, p.k);
+            stream_piece<X_TYPE, PIECES>(p, row, e, true, h[0], r, sums);
         }
     }
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-    if (blockDim.x > 32) {
-        const int warps = blockDim.x >> 5, lane = threadIdx.x & 31;
-        if (lane == 0) part[threadIdx.x >> 5] = sum;
+    double sum = sums[0] + sums[1];
+    for (int off = (lanes < 32 ? lanes : 32) / 2; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+    if (lanes > 32) {
+        const int warps = blockDim.x >> 5;
+        if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = sum;
         __syncthreads();
-        sum = lane < warps ? part[lane] : 0.0;
+        double all[4] = {0.0, 0.0, 0.0, 0.0};
+        for (int i = 0; i < warps; i += 4)
 #pragma unroll
-        for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+            for (int j = 0; j < 4; ++j)
+                if (i + j < warps) all[j] += part[i + j];
+        sum = (all[0] + all[1]) + (all[2] + all[3]);
     }
-    const float inv = (float)(1.0 / sqrt(sum / (double)p.k + p.eps));
+    const float inv = inverse_root(sum * p.per_k + p.eps);
+    const int warp_e = e0 - (lanes < 32 ? t : t & 31) * 8;  // of the warp's first lane on the row
     if constexpr (OCTETS > 0) {
 #pragma unroll
         for (int i = 0; i < N; ++i)
-            if (warp_e + i * step < p.k) output_octet(p, row, e0 + i * step, e0 + i * step < p.k, inv, v[i]);
+            if (warp_e + i * step < p.k) {
+                float v[8];
+                h[i].get(v);
+                output_octet<X_TYPE, PIECES>(p, row, e0 + i * step, has_row && e0 + i * step < p.k, inv, v);
+            }
     } else {
         for (int e = e0, we = warp_e; we < p.k; e += step, we += step) {
             const bool live = e < p.k;
+            float v[8];
             if (live) {
                 // plain loads: h was written by this thread a moment ago
                 const void *src = p.r ? p.h : p.x;
                 const int64_t base = row * (p.r ? (int64_t)p.k : p.ldx) + e;
                 for (int i = 0; i < 8; ++i) {
-                    if (e + i >= p.k) v[0][i] = 0.0f;
-                    else if (p.x_type == LLOOM_F32) v[0][i] = reinterpret_cast<const volatile float *>(src)[base + i];
+                    if (e + i < 0 || e + i >= p.k) v[i] = 0.0f;
+                    else if (X_TYPE == LLOOM_F32) v[i] = reinterpret_cast<const volatile float *>(src)[base + i];
                     else {
                         const unsigned short b = reinterpret_cast<const volatile unsigned short *>(src)[base + i];
-                        v[0][i] = p.x_type == LLOOM_F16 ? f16_bits_to_f32(b) : __uint_as_float((uint32_t)b << 16);
+                        v[i] = X_TYPE == LLOOM_F16 ? f16_bits_to_f32(b) : __uint_as_float((uint32_t)b << 16);
                     }
                 }
             }
-            output_octet(p, row, e, live, inv, v[0]);
+            output_octet<X_TYPE, PIECES>(p, row, e, live, inv, v);
         }
     }
+}
+
+using NormKernel = void (*)(NormParams);
+template <int X_TYPE, int PIECES>
+NormKernel norm_kernel(int octets) {
+    switch (octets) {
+    case 1: return rms_norm_kernel<X_TYPE, 1, PIECES>;
+    case 2: return rms_norm_kernel<X_TYPE, 2, PIECES>;
+    case 4: return rms_norm_kernel<X_TYPE, 4, PIECES>;
+    }
+    return rms_norm_kernel<X_TYPE, 0, PIECES>;
+}
+template <int X_TYPE>
+NormKernel norm_kernel(int octets, int pieces) {
+    return pieces == kWhole ? norm_kernel<X_TYPE, kWhole>(octets) : pieces == kEdges ? norm_kernel<X_TYPE, kEdges>(octets) : norm_kernel<X_TYPE, kAnywhere>(octets);
 }
 
 // Activation blocks back to the values they stand for, eight elements per thread
@@ -232,29 +341,34 @@ int rms_norm(const void *x, const void *residual, const void *weight, int x_type
     p.w = weight;
     p.h = h;
     p.y = y;
-    p.x_type = x_type;
     p.w_type = w_type;
     p.y_type = y_type;
     p.m = m;
     p.k = (int)k;
     p.ldx = ldx;
     p.ldr = ldr;
+    p.per_k = 1.0 / (double)k;
     p.eps = eps;
-    p.vec = k % 8 == 0 && aligned(x, 16) && ldx * es % 16 == 0 && aligned(weight, 16) && (blocks || aligned(y, 16)) &&
-            (!residual || (aligned(residual, 16) && ldr * es % 16 == 0 && aligned(h, 16)));
-    // One octet per thread and a row per CTA; rows of up to 256 elements get a warp, eight of them in a CTA.
-    const int64_t octets = (k + 7) / 8;
-    int threads = 32, rows = 8;
-    if (octets > 32) {
-        rows = 1;
-        threads = octets >= 1024 ? 1024 : (int)((octets + 31) / 32 * 32);
-    }
-    const int64_t per = (octets + threads - 1) / threads;
-    const dim3 grid((unsigned)((m + rows - 1) / rows));
-    auto kern = per == 1 ? rms_norm_kernel<1> : per == 2 ? rms_norm_kernel<2> : per <= 4 ? rms_norm_kernel<4> : rms_norm_kernel<0>;
+    // rows alike modulo 16 bytes: one start, and one distance between rows (or distances that are multiples of 16 bytes)
+    auto phase = [](const void *q) { return (uintptr_t)q & 15; };
+    const bool steps = (ldx - k) * es % 16 == 0 && (!residual || (ldr - k) * es % 16 == 0);
+    const bool wide = blocks ? phase(x) == 0 && ldx * es % 16 == 0 && (!residual || (phase(residual) == 0 && phase(h) == 0 && ldr * es % 16 == 0))
+                             : steps && phase(y) == phase(x) && (!residual || (phase(residual) == phase(x) && phase(h) == phase(x)));
+    // Threads: a piece each and a row per CTA, so that a row alone waits for memory once.  Many rows of halves: two pieces each, in 40 registers, so
+    // that six rows of 4096 are in flight on an SM instead of four (2048 x 4096 bf16: 12.0 us, one piece each 15.8; 592 rows: level).  (With
+    // f32 four rows in flight are enough: 22.6 us are 5.9 TB/s.)  Rows of up to 32 pieces share a CTA of 256 threads.
+    const int pieces = !wide ? kAnywhere : phase(x) == 0 && phase(weight) == 0 && k % 8 == 0 && ldx * es % 16 == 0 ? kWhole : kEdges;
+    const int64_t octets = (k + 7) / 8 + (pieces == kEdges ? 1 : 0);
+    const bool pairs = x_type != LLOOM_F32 && m >= 592 && octets > 64 && octets <= 1024;
+    const int per = pairs ? 2 : octets <= 1024 ? 1 : octets <= (x_type == LLOOM_F32 ? 2048 : 1024) ? 2 : octets <= 4096 ? 4 : 0;
+    const int64_t threads = per ? (octets + per - 1) / per : 1024;
+    p.lanes = threads > 32 ? 0 : threads <= 8 ? 8 : threads <= 16 ? 16 : 32;
+    const unsigned block = p.lanes ? 256 : (unsigned)((threads + 31) / 32 * 32);
+    const unsigned grid = p.lanes ? (unsigned)ceil_div64(m, 256 / p.lanes) : (unsigned)m;
+    auto kern = x_type == LLOOM_F32 ? norm_kernel<LLOOM_F32>(per, pieces) : x_type == LLOOM_F16 ? norm_kernel<LLOOM_F16>(per, pieces) : norm_kernel<LLOOM_BF16>(per, pieces);
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = dim3((unsigned)threads, (unsigned)rows);
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(block);
     cfg.stream = (cudaStream_t)stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

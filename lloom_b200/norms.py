@@ -18,14 +18,16 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, residual:
     ``x`` and ``residual`` are f32, f16 or bf16, of one type and shape, contiguous or matrices with contiguous rows; ``weight``
     has any of the three types.  The blocks are those of the f32 values of ``y``, whose every rounding is defined, so they do
     not depend on how a row is summed."""
-    got = _native().rms_norm(x, weight, eps, residual, -1 if act_for is None else act_type(act_for))
+    act = None if act_for is None else act_type(act_for)
+    got = _native().rms_norm(x, weight, eps, residual, -1 if act is None else act)
     if got is None:
         _refuse(x, weight, residual, act_for)
-    if act_for is None:
+    if act is None:
         return got
+    shape = tuple(x.shape)
     if residual is None:
-        return QActs(got, act_type(act_for))
-    return QActs(got[0], act_type(act_for)), got[1]
+        return QActs._own(got, act, shape)
+    return QActs._own(got[0], act, shape), got[1]
 
 
 def _refuse(x, weight, residual, act_for):

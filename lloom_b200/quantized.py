@@ -337,8 +337,10 @@ class QTensor:
 
 
 _ELEM_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}
-_ACT_TYPES = {GgmlDType.Q4_0: GgmlDType.Q8_0, GgmlDType.Q5_0: GgmlDType.Q8_0, GgmlDType.Q8_0: GgmlDType.Q8_0,
-              GgmlDType.Q4K: GgmlDType.Q8K, GgmlDType.Q5K: GgmlDType.Q8K, GgmlDType.Q6K: GgmlDType.Q8K}
+# the activation block type of every weight type (VecDotType), kept on the members: a dictionary would hash their names at each call
+for _t in _WEIGHT_TYPES:
+    _t.act = GgmlDType.Q8K if _t.name.endswith("K") else GgmlDType.Q8_0
+_ACT_BLOCK = {int(GgmlDType.Q8_0): (32, 34), int(GgmlDType.Q8K): (256, 292)}
 
 
 class QActs:
@@ -352,11 +354,18 @@ class QActs:
         dtype = GgmlDType(dtype)
         if dtype not in (GgmlDType.Q8_0, GgmlDType.Q8K):
             raise LloomError(_lib.ERR_DTYPE, "QActs", f"{dtype!r} is not an activation block type")
-        be, bb = _ACT_BLOCK[dtype]
+        be, bb = _ACT_BLOCK[int(dtype)]
         if blocks.dtype != torch.uint8 or blocks.dim() < 1 or blocks.shape[-1] % bb != 0:
             raise LloomError(_lib.ERR_SHAPE, "QActs", f"{tuple(blocks.shape)} {blocks.dtype} is not rows of {dtype!r} blocks")
         self.blocks, self.dtype = blocks, dtype
         self.shape = (*blocks.shape[:-1], blocks.shape[-1] // bb * be)
+
+    @classmethod
+    def _own(cls, blocks: torch.Tensor, dtype: GgmlDType, shape: tuple) -> "QActs":
+        """Of blocks that this package has made."""
+        a = cls.__new__(cls)
+        a.blocks, a.dtype, a.shape = blocks, dtype, shape
+        return a
 
     @classmethod
     def quantize(cls, x: torch.Tensor, act_for: GgmlDType) -> "QActs":
@@ -372,12 +381,9 @@ class QActs:
         return out
 
 
-_ACT_BLOCK = {GgmlDType.Q8_0: (32, 34), GgmlDType.Q8K: (256, 292)}
-
-
 def act_type(w_dtype: GgmlDType) -> GgmlDType:
     """The activation block type that weights of this type are dotted with."""
-    t = _ACT_TYPES.get(w_dtype)
+    t = getattr(w_dtype, "act", None)
     if t is None:
         raise LloomError(_lib.ERR_DTYPE, "act_type", f"{w_dtype!r} is not a weight type of this backend")
     return t
@@ -407,7 +413,7 @@ class QMatMul:
         result is that of ``forward`` on f32 values that quantize to these blocks, bit for bit.  ``dtype``: of the result."""
         qt = self.qtensor
         n, k = qt.shape
-        if acts.dtype != _ACT_TYPES[qt.dtype()] or acts.shape[-1] != k:
+        if acts.dtype is not qt.dtype().act or acts.shape[-1] != k:
             raise LloomError(_lib.ERR_SHAPE, "forward_quantized",
                              f"{acts.dtype!r} activations {tuple(acts.shape)} do not fit {qt.dtype()!r} weights {(n, k)}")
         if dtype not in _ELEM_TYPES:
@@ -461,7 +467,7 @@ def forward_group(mats: Sequence["QMatMul"], xs: "torch.Tensor | QActs", stores:
     tensors = [mm.qtensor for mm in mats]
     k = tensors[0].shape[1]
     blocks = isinstance(xs, QActs)
-    if all(t.shape[1] == k for t in tensors) and not (blocks and xs.dtype != _ACT_TYPES[tensors[0].dtype()]):
+    if all(t.shape[1] == k for t in tensors) and not (blocks and xs.dtype is not tensors[0].dtype().act):
         got = _native().group([t.storage._native for t in tensors], [t.shape[0] for t in tensors], k, xs.blocks if blocks else xs,
                               None if stores is None else list(stores), None if outs is None else list(outs), blocks)
         if got is not None:

@@ -160,41 +160,52 @@ __global__ void __launch_bounds__(256) mx_to_blocks_kernel(const uint8_t *__rest
         blk[1 + j] = (uint8_t)(((w[j >> 3] >> (4 * (j & 7))) & 15u) | (((w[2 + (j >> 3)] >> (4 * (j & 7))) & 15u) << 4));
 }
 
-// Eight elements per thread.  2^e of the smallest scales is subnormal: the product with an element's value is exact all the same.
+// A code's value times the scale: its exponent (bias 1) and mantissa bits, moved to the places of f16's, read as the value times 2^-14.
+__device__ __forceinline__ float mx_value(uint32_t code, float d) {
+    const uint32_t half = ((code & 7u) << 9) | ((code & 8u) << 12);
+    return __fmul_rn(__half2float(__ushort_as_half((unsigned short)half)) * 16384.0f, d);
+}
+
+// Image to values: a warp has two units of a row, as in the quantizer.  2^e of the smallest scale is subnormal: products with it are exact all
+// the same.
 template <bool F16>
-__global__ void __launch_bounds__(256) mx_dequantize_kernel(const uint8_t *__restrict__ image, int64_t n, int k, int units, void *__restrict__ out) {
+__global__ void __launch_bounds__(256) mx_dequantize_kernel(const uint8_t *__restrict__ image, int n, int k, int units, int across, void *__restrict__ out) {
     launch_dependents();
     wait_predecessor();
-    const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-    const int per_row = k / 8;
-    const int64_t row = i / per_row;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int row = (int)blockIdx.x * (8 / across) + warp / across, u0 = ((int)blockIdx.y * across + warp % across) * kQuantUnits;
     if (row >= n) return;
-    const int e = (int)(i - row * per_row) * 8, b = e / kMxBlock, c = b & 7, r = (int)(row % kMxTile);
-    const uint8_t *unit = image + (row / kMxTile * units + (b >> 3)) * (int64_t)mx_unit_bytes(kMxTile);
-    const uint32_t q = *reinterpret_cast<const uint32_t *>(unit + mx_chunk_offset(r, c) + ((e >> 3) & 3) * 4);
-    const uint32_t s = unit[mx_scale_offset(kMxTile, r, c)];
-    const float d = s == 255u ? __uint_as_float(0x7fc00000u) : s == 0u ? __uint_as_float(0x00400000u) : __uint_as_float(s << 23);
-    float v[8];
+    const int r = row % kMxTile, c = lane >> 2;
+    const uint8_t *unit = image + ((int64_t)(row / kMxTile) * units + u0) * mx_unit_bytes(kMxTile);
+    const int chunk = mx_chunk_offset(r, c) + (lane & 3) * 4, scale = mx_scale_offset(kMxTile, r, c);
+    uint32_t q[kQuantUnits], s[kQuantUnits];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const uint32_t code = (q >> (4 * j)) & 15u, m = code & 7u;
-        // twice the magnitude: 0, 1, 2, 3, 4, 6, 8, 12
-        const uint32_t twice = m < 4u ? m : m == 4u ? 4u : m == 5u ? 6u : m == 6u ? 8u : 12u;
-        const float a = 0.5f * (float)twice;
-        v[j] = __fmul_rn(code & 8u ? -a : a, d);
+    for (int j = 0; j < kQuantUnits; ++j) {
+        const bool in = (u0 + j) * kMxUnit + lane * 8 < k;
+        q[j] = in ? __ldg(reinterpret_cast<const uint32_t *>(unit + j * mx_unit_bytes(kMxTile) + chunk)) : 0u;
+        s[j] = in ? __ldg(unit + j * mx_unit_bytes(kMxTile) + scale) : 0u;
     }
-    if (F16) {
-        uint32_t h[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const __half2 t = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
-            h[j] = *reinterpret_cast<const uint32_t *>(&t);
+    for (int j = 0; j < kQuantUnits; ++j) {
+        const int e = (u0 + j) * kMxUnit + lane * 8;
+        if (e >= k) continue;
+        const float d = s[j] == 255u ? __uint_as_float(0x7fc00000u) : s[j] == 0u ? __uint_as_float(0x00400000u) : __uint_as_float(s[j] << 23);
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = mx_value(q[j] >> (4 * i), d);
+        if (F16) {
+            uint32_t h[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const __half2 t = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+                h[i] = *reinterpret_cast<const uint32_t *>(&t);
+            }
+            *reinterpret_cast<uint4 *>(reinterpret_cast<__half *>(out) + (int64_t)row * k + e) = make_uint4(h[0], h[1], h[2], h[3]);
+        } else {
+            float4 *o = reinterpret_cast<float4 *>(reinterpret_cast<float *>(out) + (int64_t)row * k + e);
+            o[0] = make_float4(v[0], v[1], v[2], v[3]);
+            o[1] = make_float4(v[4], v[5], v[6], v[7]);
         }
-        *reinterpret_cast<uint4 *>(reinterpret_cast<__half *>(out) + row * k + e) = make_uint4(h[0], h[1], h[2], h[3]);
-    } else {
-        float4 *o = reinterpret_cast<float4 *>(reinterpret_cast<float *>(out) + row * k + e);
-        o[0] = make_float4(v[0], v[1], v[2], v[3]);
-        o[1] = make_float4(v[4], v[5], v[6], v[7]);
     }
 }
 
@@ -729,13 +740,18 @@ int mx_check(int64_t m, int64_t n, int64_t k) {
 
 int64_t mx_image_bytes(int64_t rows, int64_t k, int T, int parts = 1) { return (rows + T - 1) / T * mx_units(k) * mx_unit_bytes(T, parts); }
 
+// CTAs of eight warps over rows of units, kQuantUnits to a warp: `across` of a CTA's warps lie along a row
+dim3 mx_row_grid(int64_t rows, int64_t units, int &across) {
+    for (across = 1; across < 8 && across * kQuantUnits < units; across *= 2) {}
+    return dim3((unsigned)ceil_div64(rows, 8 / across), (unsigned)ceil_div64(units, kQuantUnits * across));
+}
+
 int launch_mx_quantize(const void *x, int x_type, int64_t m, int64_t k, int T, int parts, uint8_t *image, bool trigger, bool overlap,
                        cudaStream_t stream) {
     const int64_t rows = (m + T - 1) / T * T, units = mx_units(k);
     if (rows > 0x7fffffff) return LLOOM_ERR_SHAPE;
-    int across = 1;
-    while (across < 8 && across * kQuantUnits < units) across *= 2;
-    const dim3 grid((unsigned)ceil_div64(rows, 8 / across), (unsigned)ceil_div64(units, kQuantUnits * across));
+    int across;
+    const dim3 grid = mx_row_grid(rows, units, across);
     if (grid.y > 65535) return LLOOM_ERR_SHAPE;
     auto kern = x_type == LLOOM_F32   ? mx_quantize_kernel<LLOOM_F32>
                 : x_type == LLOOM_F16 ? mx_quantize_kernel<LLOOM_F16>
@@ -918,10 +934,11 @@ int mx_dequantize(const void *image, int64_t rows, int64_t k, void *out, bool f1
     if (rc != LLOOM_OK) return rc;
     if (!image || !out) return LLOOM_ERR_NULL;
     if (!aligned(image, 256) || !aligned(out, 16)) return LLOOM_ERR_ALIGN;
-    const int64_t grid = ceil_div64(rows * (k / 8), 256);
-    if (grid > 0x7fffffff) return LLOOM_ERR_SHAPE;
-    return launch_status(launch_early(f16 ? mx_dequantize_kernel<true> : mx_dequantize_kernel<false>, (unsigned)grid, 256, 0, overlap,
-                                      (cudaStream_t)stream, (const uint8_t *)image, rows, (int)k, (int)mx_units(k), out));
+    int across;
+    const dim3 grid = mx_row_grid(rows, mx_units(k), across);
+    if (grid.y > 65535) return LLOOM_ERR_SHAPE;
+    return launch_status(launch_early(f16 ? mx_dequantize_kernel<true> : mx_dequantize_kernel<false>, grid, 256, 0, overlap, (cudaStream_t)stream,
+                                      (const uint8_t *)image, (int)rows, (int)k, (int)mx_units(k), across, out));
 }
 
 }  // namespace lloom

@@ -11,6 +11,7 @@
 // the blocks are known to be in place (nothing writes them after the upload), and later forwards may stream them while the
 // stream's previous kernel is still finishing.  A storage whose device pointer has been handed out, or that was made over a
 // caller's tensor, stays with the first kind: the holder may write through it.
+#include <torch/csrc/Device.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/extension.h>
 
@@ -41,13 +42,17 @@ PyObject *fail(int status, const char *where) {
 }
 
 // Grow-only scratch per (device, stream): launches on different streams never share a buffer.  A buffer that has been
-// outgrown stays alive: a CUDA graph captured earlier may hold its address.
+// outgrown stays alive: a CUDA graph captured earlier may hold its address.  A call that is being captured gets memory of its own, which its graph
+// keeps: graphs captured on one stream may be replayed side by side on others.
 struct Workspaces {
     std::mutex mu;
     std::map<std::pair<int, cudaStream_t>, at::Tensor> bufs;
     std::vector<at::Tensor> retired;
 
-    const at::Tensor &get(c10::Device dev, cudaStream_t stream, int64_t bytes) {
+    at::Tensor get(c10::Device dev, cudaStream_t stream, int64_t bytes) {
+        cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+        if (cudaStreamIsCapturing(stream, &capture) == cudaSuccess && capture != cudaStreamCaptureStatusNone)
+            return at::detail::empty_cuda({std::max<int64_t>(bytes, 512)}, at::kByte, dev, std::nullopt);
         std::lock_guard<std::mutex> lock(mu);
         at::Tensor &buf = bufs[{dev.index(), stream}];
         if (!buf.defined() || buf.numel() < bytes) {
@@ -206,7 +211,7 @@ PyObject *Storage_forward(PyObject *o, PyObject *const *args, Py_ssize_t nargs) 
                                : lloom_b200_workspace_bytes(self->dtype, m, n, k);
     if (need <= 0) Py_RETURN_NONE;
     const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
-    const at::Tensor &ws = workspaces().get(dev, stream, need);
+    const at::Tensor ws = workspaces().get(dev, stream, need);
     const int rc = lloom::qmatmul_forward(self->dtype, self->data->const_data_ptr(),
                                           image ? static_cast<char *>(self->image->data_ptr()) + self->image_off : nullptr,
                                           x.const_data_ptr(), yp, m, n, k, ldy, store, ws.data_ptr(), ws.numel(), stream, io);
@@ -250,7 +255,7 @@ PyObject *Storage_forward_acts(PyObject *o, PyObject *const *args, Py_ssize_t na
     io.overlap = overlaps(self);
     io.y_type = y_type;
     const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
-    const at::Tensor &ws = workspaces().get(dev, stream, need);
+    const at::Tensor ws = workspaces().get(dev, stream, need);
     const int rc = lloom::qmatmul_forward_acts(self->dtype, self->data->const_data_ptr(),
                                                image ? static_cast<char *>(self->image->data_ptr()) + self->image_off : nullptr,
                                                a.const_data_ptr(), y.data_ptr(), m, n, k, n, ws.data_ptr(), ws.numel(), stream, io);
@@ -307,7 +312,7 @@ PyObject *Storage_experts(PyObject *o, PyObject *const *args, Py_ssize_t nargs) 
     const int64_t need = lloom_b200_workspace_bytes(self->dtype, 1, n, k);
     if (need <= 0) Py_RETURN_NONE;
     const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
-    const at::Tensor &ws = workspaces().get(dev, stream, need);
+    const at::Tensor ws = workspaces().get(dev, stream, need);
     FwdIo io;
     io.overlap = overlaps(self);
     const int rc = lloom::indexed_moe_forward(self->dtype, self->data->const_data_ptr(), n_experts, n, k, x.const_data_ptr<float>(),
@@ -382,7 +387,7 @@ PyObject *module_group(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
         PyList_SET_ITEM(list.get(), g, item);
     }
     const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
-    const at::Tensor &ws = workspaces().get(dev, stream, need);
+    const at::Tensor ws = workspaces().get(dev, stream, need);
     const int rc = lloom::qmatmul_forward_group(st[0]->dtype, (int)G, w, blocks ? x.const_data_ptr() : nullptr,
                                                 blocks ? nullptr : x.const_data_ptr(), y, n, ld, store, m, k, ws.data_ptr(),
                                                 ws.numel(), stream, io);
@@ -468,6 +473,13 @@ PyObject *module_mx_from_blocks(PyObject *, PyObject *const *args, Py_ssize_t na
     END_HANDLE_TH_ERRORS
 }
 
+// shape() -> (n, k)
+PyObject *MxStorage_shape(PyObject *o, PyObject *) {
+    return Py_BuildValue("LL", (long long)reinterpret_cast<MxStorage *>(o)->n, (long long)reinterpret_cast<MxStorage *>(o)->k);
+}
+// device() -> torch.device
+PyObject *MxStorage_device(PyObject *o, PyObject *) { return THPDevice_New(reinterpret_cast<MxStorage *>(o)->image->device()); }
+
 // to_blocks() -> uint8 [n, k / 32 * 17] on the GPU
 PyObject *MxStorage_to_blocks(PyObject *o, PyObject *) {
     HANDLE_TH_ERRORS
@@ -514,7 +526,7 @@ PyObject *MxStorage_forward(PyObject *o, PyObject *const *args, Py_ssize_t nargs
     sizes.back() = self->n;
     at::Tensor y = at::detail::empty_cuda(sizes, x.scalar_type(), dev, std::nullopt);
     const cudaStream_t stream = stream_of(dev);
-    const at::Tensor &ws = workspaces().get(dev, stream, need);
+    const at::Tensor ws = workspaces().get(dev, stream, need);
     const int mode = lloom::launch_overlap();
     const int rc = lloom::mx_forward(self->image->const_data_ptr(), x.const_data_ptr(), x_type, y.data_ptr(), x_type, m, self->n, self->k,
                                      self->n, ws.data_ptr(), ws.numel(), stream, mode > 0 || (mode < 0 && self->settled));
@@ -678,6 +690,8 @@ PyMethodDef storage_methods[] = {{"forward", FAST(Storage_forward), METH_FASTCAL
 PyMethodDef mx_methods[] = {{"forward", FAST(MxStorage_forward), METH_FASTCALL, nullptr},
                             {"dequantize", MxStorage_dequantize, METH_O, nullptr},
                             {"to_blocks", MxStorage_to_blocks, METH_NOARGS, nullptr},
+                            {"shape", MxStorage_shape, METH_NOARGS, nullptr},
+                            {"device", MxStorage_device, METH_NOARGS, nullptr},
                             {nullptr, nullptr, 0, nullptr}};
 
 PyMethodDef module_methods[] = {{"group", FAST(module_group), METH_FASTCALL, nullptr},

@@ -21,8 +21,14 @@ class MxTensor:
     """A matrix ``[n, k]`` of microscaled 4-bit values on the GPU, k a multiple of 32, laid out for the tensor cores (4.25 bits
     an element, rows padded to 128 and k to 256)."""
 
-    def __init__(self, native, shape: Sequence[int], device: torch.device):
-        self._native, self.shape, self._device = native, tuple(int(s) for s in shape), device
+    __slots__ = ("_native",)
+
+    def __init__(self, native):
+        self._native = native
+
+    @property
+    def shape(self) -> tuple:
+        return self._native.shape()
 
     @classmethod
     def quantize(cls, src: torch.Tensor) -> "MxTensor":
@@ -31,7 +37,7 @@ class MxTensor:
         st = _native().mx_quantize(src)
         if st is None:
             _refuse("MxTensor.quantize", src, src.shape[-1] if src.dim() else 0, None)
-        return cls(st, (src.numel() // src.shape[-1], src.shape[-1]), src.device)
+        return cls(st)
 
     @classmethod
     def from_data(cls, data, shape: Sequence[int], device="cuda") -> "MxTensor":
@@ -56,14 +62,15 @@ class MxTensor:
         st = _native().mx_from_blocks(blocks, shape)
         if st is None:
             raise LloomError(_lib.ERR_SHAPE, "MxTensor.from_data", f"unsupported shape {shape}")
-        return cls(st, shape, blocks.device)
+        return cls(st)
 
     def device(self) -> torch.device:
-        return self._device
+        return self._native.device()
 
     def storage_size_in_bytes(self) -> int:
         """Of the blocks; the image takes the padding on top."""
-        return self.shape[0] * self.shape[1] // MX_BLOCK * MX_BLOCK_BYTES
+        n, k = self.shape
+        return n * k // MX_BLOCK * MX_BLOCK_BYTES
 
     def data(self) -> bytes:
         """The blocks as a file stores them."""

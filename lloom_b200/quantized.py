@@ -384,6 +384,8 @@ class QActs:
 def act_type(w_dtype: GgmlDType) -> GgmlDType:
     """The activation block type that weights of this type are dotted with."""
     t = getattr(w_dtype, "act", None)
+    if t is None and not isinstance(w_dtype, GgmlDType):  # a type id
+        t = getattr(GgmlDType.from_u32(w_dtype), "act", None)
     if t is None:
         raise LloomError(_lib.ERR_DTYPE, "act_type", f"{w_dtype!r} is not a weight type of this backend")
     return t

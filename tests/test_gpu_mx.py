@@ -262,3 +262,61 @@ def test_gguf_tensor(dev):
     t = G.Content.read(f).tensor(f, "w", dev)
     assert isinstance(t, MxTensor) and t.shape == (40, 96)
     assert torch.equal(MxMatMul.from_tensor(t).forward(x.to(dev)).cpu().double(), x.double() @ w.double().T)
+
+
+def test_graphs_side_by_side(dev):
+    """Two graphs captured on one stream, replayed together on others: neither touches the other's activations."""
+    from lloom_b200 import MxMatMul, MxTensor
+
+    mats = [MxMatMul.from_tensor(MxTensor.quantize(whole(i, 4096, 4096).to(dev))) for i in (1, 2)]
+    xs = [whole(i + 5, 100, 4096).to(dev) for i in (1, 2)]
+    want = [mm.forward(x) for mm, x in zip(mats, xs)]
+    side = torch.cuda.Stream()
+    graphs, outs = [], []
+    for mm, x in zip(mats, xs):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            outs.append([mm.forward(x) for _ in range(4)])
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in graphs]
+    torch.cuda.synchronize()
+    for _ in range(30):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    for w, o in zip(want, outs):
+        assert all(torch.equal(w, y) for y in o)
+
+
+@pytest.mark.parametrize("m", [3, 40, 200])
+@pytest.mark.parametrize("y_type", [0, 1, 30])
+def test_c_entry_row_distance_and_types(dev, m, y_type):
+    """Rows of outputs further apart than they are long, results of another type than the activations; what lies between stays."""
+    from lloom_b200 import _lib
+
+    L = _lib.lib()
+    n, k, ldy = 130, 512, 137
+    w, x = whole(1, n, k).to(dev), whole(2, m, k).half().to(dev)
+    image = torch.zeros(L.lloom_b200_mx_image_bytes(n, k), dtype=torch.uint8, device=dev)
+    ws = torch.empty(L.lloom_b200_mx_workspace_bytes(m, n, k), dtype=torch.uint8, device=dev)
+    t = {0: torch.float32, 1: torch.float16, 30: torch.bfloat16}[y_type]
+    y = torch.full((m, ldy), 77.0, dtype=t, device=dev)
+    stream = torch.cuda.current_stream().cuda_stream
+    assert L.lloom_b200_mx_quantize(w.data_ptr(), 0, n, k, image.data_ptr(), image.numel(), stream) == 0
+    assert L.lloom_b200_mx_fwd(image.data_ptr(), x.data_ptr(), 1, y.data_ptr(), y_type, m, n, k, ldy, ws.data_ptr(), ws.numel(), stream) == 0
+    torch.cuda.synchronize()
+    assert torch.equal(y[:, :n].cpu(), (x.cpu().double() @ w.cpu().double().T).to(t))
+    assert (y[:, n:] == 77).all()
+
+
+def test_plans_agree(dev):
+    """The kernels for few rows, for some and for pairs of CTAs, and their ways of cutting K and the rows: one row's bits where sums are exact."""
+    from lloom_b200 import MxMatMul, MxTensor
+
+    for n, k in ((300, 8192), (1100, 16384)):
+        w, x = whole(n, n, k), whole(3, 520, k)
+        mm = MxMatMul.from_tensor(MxTensor.quantize(w.to(dev)))
+        want = (x.double() @ w.double().T).float()
+        for m in (1, 2, 4, 16, 17, 65, 128, 129, 250, 384, 520):
+            assert torch.equal(mm.forward(x[:m].to(dev)).cpu(), want[:m]), (n, k, m)

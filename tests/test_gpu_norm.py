@@ -232,3 +232,38 @@ def test_decode_step(dev, fmt, m):
     forward_group([up], acts2, stores=[2], outs=[g2])
     assert torch.equal(hidden, g2)
     assert torch.equal(down.forward(hidden), down.forward(g2))
+
+
+@pytest.mark.parametrize("k", [64, 1000, 4099, 40000])
+def test_stream_updated_in_place(dev, k):
+    """The C entry with h in the residual's own buffer, rows of x further apart, and weights of another type."""
+    from lloom_b200 import _lib
+
+    L = _lib.lib()
+    a, r, w = inputs(k, 5, k, torch.float16, torch.float32)
+    x = torch.zeros(5, k + 24, dtype=torch.float16, device=dev)
+    x[:, :k] = a.to(dev)
+    h, y = r.to(dev), torch.empty(5, k, dtype=torch.float16, device=dev)
+    wd = w.to(dev)
+    assert L.lloom_b200_rms_norm(x.data_ptr(), h.data_ptr(), wd.data_ptr(), 1, 0, EPS, 5, k, k + 24, k, h.data_ptr(), y.data_ptr(), 1,
+                                 torch.cuda.current_stream().cuda_stream) == 0
+    torch.cuda.synchronize()
+    assert torch.equal(h.cpu(), steps(a, r, w)[0])
+    check_values(y, a, r, w)
+
+
+@pytest.mark.parametrize("x", ["f16", "f32"])
+@pytest.mark.parametrize("m,k", [(700, 1000), (600, 4097), (640, 8192), (600, 8200), (1500, 40), (9, 72)])
+def test_many_rows(dev, m, k, x):
+    """Two pieces per thread, rows that share a CTA, rows off the boundary among many."""
+    from lloom_b200 import rms_norm
+
+    a, r, w = inputs(m + k, m, k, TYPES[x])
+    y, h = rms_norm(a.to(dev), w.to(dev), EPS, r.to(dev))
+    assert torch.equal(h.cpu(), steps(a, r, w)[0])
+    check_values(y, a, r, w)
+    # from a base off the boundary, alike for all
+    z = torch.zeros(2, m * k + 3, dtype=a.dtype, device=dev)
+    z[0, 3:], z[1, 3:] = a.view(-1).to(dev), r.view(-1).to(dev)
+    y2, h2 = rms_norm(z[0, 3:].view(m, k), w.to(dev), EPS, z[1, 3:].view(m, k))
+    assert torch.equal(y, y2) and torch.equal(h, h2)

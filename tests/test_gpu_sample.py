@@ -229,3 +229,38 @@ def test_output_head_then_draw_captured(dev):
         assert torch.equal(got[0], want) and torch.equal(got[1], want_p)
         for r in range(b):
             assert got[0][r] == draw(logits[r].cpu().numpy(), float(u[r]), 0.8, 100, 0.9, 0.0)[0]
+
+
+def test_c_entry(dev):
+    """Rows apart, no probabilities wanted, settings of every kind; streams side by side."""
+    from lloom_b200 import _lib
+
+    L = _lib.lib()
+    b, v = 6, 5003
+    logits, u = rand(9, b, v, torch.float16)
+    wide = torch.full((b, v + 13), 60000.0, dtype=torch.float16, device=dev)
+    wide[:, :v] = logits.to(dev)
+    ud, k = torch.from_numpy(u).to(dev), torch.full((b,), 33, dtype=torch.int32, device=dev)
+    want = [draw(logits[i].float().numpy(), np.float64(u[i]), 0.9, 33, 0.8, 0.0)[0] for i in range(b)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    outs = [torch.full((b + 1,), -5, dtype=torch.int64, device=dev) for _ in range(32)]
+    torch.cuda.synchronize()
+    for i, ids in enumerate(outs):
+        assert L.lloom_b200_sample(wide.data_ptr(), 1, b, v, v + 13, ud.data_ptr(), None, 0.9, k.data_ptr(), 0, None, 0.8, None, 0.0, ids.data_ptr(),
+                                   None, streams[i % 4].cuda_stream) == 0
+    torch.cuda.synchronize()
+    for ids in outs:
+        assert ids.tolist() == want + [-5]
+
+
+def test_least_temperature(dev):
+    """Temperatures down to 2^-120 are computed with, below that the first of the largest is taken; a temperature without end draws evenly."""
+    logits = torch.tensor([[1.0, 3.0, 3.0, 2.0]] * 3)
+    u = np.array([0.1, 0.6, 0.9])
+    check(dev, logits, u, t=2.0 ** -119)
+    check(dev, logits, u, t=float("inf"))
+    import lloom_b200 as lb
+
+    ids, probs = lb.sample(logits.to(dev), torch.from_numpy(u.astype(np.float32)).to(dev), temperature=2.0 ** -121)
+    assert ids.tolist() == [1, 1, 1] and probs.tolist() == [1.0, 1.0, 1.0]

@@ -221,7 +221,7 @@ int lloom_b200_qmatmul_fwd_group(int w_dtype, int n_mats, const void *const *w_b
  * activation blocks [m][k / block], those of lloom_b200_quantize_act on the f32 values of y.  The mean and 1 / sqrt are
  * computed in 64 bits and rounded once, then h * (1 / sqrt) and the product with the weight are rounded to f32 each.
  * x, residual: [m] rows of k elements of x_type, ldx / ldr elements apart; weight: k elements of w_type; h, y: contiguous.
- * `h` may be the residual's own buffer where ldr == k; nothing else may overlap.  Types: LLOOM_F32, LLOOM_F16, LLOOM_BF16.
+ * `h` may be the residual's own buffer where ldr == k (refused otherwise); nothing else may overlap.  Types: LLOOM_F32, LLOOM_F16, LLOOM_BF16.
  * Pointers are aligned to their elements, blocks to 4 bytes; rows and weights on 16 bytes with k a multiple of 8 are read faster. */
 int lloom_b200_rms_norm(const void *x, const void *residual, const void *weight, int x_type, int w_type, double eps, int64_t m, int64_t k,
                         int64_t ldx, int64_t ldr, void *h, void *y, int y_type, void *stream);

@@ -329,7 +329,7 @@ int rms_norm(const void *x, const void *residual, const void *weight, int x_type
              int64_t ldr, void *h, void *y, int y_type, void *stream, bool overlap) {
     const bool blocks = y_type == LLOOM_Q8_0 || y_type == LLOOM_Q8_K;
     if (!elem_type_ok(x_type) || !elem_type_ok(w_type) || (!blocks && y_type != x_type)) return LLOOM_ERR_DTYPE;
-    if (m <= 0 || k <= 0 || m > 0x7fffffff || k > (1 << 24) || ldx < k || (residual && ldr < k)) return LLOOM_ERR_SHAPE;
+    if (m <= 0 || k <= 0 || m > 0x7fffffff || k > (1 << 24) || ldx < k || (residual && (ldr < k || (h == residual && ldr != k)))) return LLOOM_ERR_SHAPE;
     if (blocks && k % lloom_b200_block_elems(y_type) != 0) return LLOOM_ERR_SHAPE;
     if (!x || !weight || !y || (residual && !h)) return LLOOM_ERR_NULL;
     const int64_t es = elem_bytes(x_type), ws = elem_bytes(w_type);

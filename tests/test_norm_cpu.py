@@ -81,3 +81,11 @@ def test_python_refuses(cuda_lib):
     assert status(mm.forward_quantized, acts, torch.float64) == _lib.ERR_DTYPE
     assert status(mm.forward_quantized, QActs(torch.zeros(4, 292, dtype=torch.uint8)[::2], GgmlDType.Q8K)) == _lib.ERR_SHAPE
     assert status(forward_group, [mm], QActs(torch.zeros(2, 34 * 8, dtype=torch.uint8), GgmlDType.Q8_0)) == _lib.ERR_SHAPE
+
+
+def test_stream_in_place_needs_rows_that_follow_each_other(cuda_lib):
+    """h is contiguous: in the residual's own buffer its rows would run over those of a wider residual before they are read."""
+    from lloom_b200 import _lib
+
+    p = 1 << 20
+    assert _lib.lib().lloom_b200_rms_norm(p, p + 65536, p, 0, 0, 1e-5, 4, 64, 64, 80, p + 65536, p + 131072, 0, None) == _lib.ERR_SHAPE

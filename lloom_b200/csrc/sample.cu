@@ -6,15 +6,19 @@
 //
 // A cluster of CTAs has a row: it is read once, stays in shared memory, and everything after works there.  A filter's border is found by
 // a histogram over 2048 buckets of (max - l) / T, 1/64 wide, then within the bucket that holds it: by further histograms over the bits of the
-// logits while it has more than 256 tokens, else by ranking them against one another; equal logits by index.  Where all tokens up to
-// the border are as few, the draw needs no more than these.  No sort of the row.
+// logits while it has more than 512 tokens, else by sorting these; equal logits by index.  Where all tokens up to the border are no more
+// than 256, the draw needs these alone.  No sort of the row.  (With 256 sorted by counting, 16 rows of 128256 at temperatures up to 1.5, whose
+// border buckets have 300 to 500 tokens, took 59 us instead of 41.)
 //
 // Weights are summed as integers, in units of 2^-43 of the largest weight: the sums are exact, so that they depend neither on
 // the split of a row nor on the order of atomics, and borders fall where 64-bit arithmetic puts them.  (In 32 bits a running sum over
 // 100,000 tokens is off by more than a token's share of it.)  Tokens below 2^-44 of the largest weight count as zero.
 // exp: table of 2^(-j/32) and a polynomial (table-driven, after Tang 1989) in 64-bit arithmetic, relative error below 5e-14.
 //
-// Bound by latency for a few rows (a launch, one read of DRAM, a handful of cluster barriers), by the 64-bit pipe and the read for many.
+// Bound by latency for a few rows: a launch, one read of DRAM, six to eight cluster barriers of about a microsecond with short passes between
+// them (1 x 128256 f32 with all filters 15.5 us, 7 x 50257 bf16 with top-p 33).  For many rows by the passes themselves: shared-memory
+// additions (nine cycles each) and 64-bit arithmetic (two cycles a warp and multiply-add) of the weights: 64 x 128256 f32, 33 MB, settings of their own, 71 us.
+// There a row read from L2 in every pass by fewer CTAs, all rows at once, was faster for alike rows (75 us for 85) and slower for unlike ones (126 for 84).
 #include <mutex>
 #include <type_traits>
 
@@ -28,7 +32,8 @@ namespace {
 
 constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kBuckets = 2048;
-constexpr int kList = 256;  // tokens that are ranked against one another
+constexpr int kList = 256;       // tokens that the draw needs alone: every one up to the border
+constexpr int kLast = kThreads;  // tokens of the border's bucket that are sorted
 constexpr int kMaxCluster = 8;
 constexpr int kMaxChunk = LLOOM_B200_MAX_VOCAB / kMaxCluster;  // logits of a CTA
 constexpr double kLeastTemperature = 7.5231638452626401e-37;  // 2^-120: 2^896 / T stays finite
@@ -59,7 +64,18 @@ struct Shared {
         struct {
             uint32_t low[kBuckets], mid[kBuckets], high[kBuckets];
         };
-        float batch[kWarps][2 * kSpan];
+        struct {
+            float batch[kWarps][2 * kSpan];
+            uint16_t place[kWarps][2 * kSpan];  // (kMaxChunk < 2^16)
+        };
+        struct {  // (`low` and `high` stay free in the draw from a list)
+            uint32_t low_[kBuckets];
+            struct alignas(16) {
+                uint2 token;  // (index, key): in order as one number
+                unsigned long long weight;
+            } list[kLast];
+            unsigned long long exchange[2][kThreads];
+        };
     };
     unsigned long long warp_w[kWarps];
     unsigned long long half_w[kList];
@@ -69,22 +85,21 @@ struct Shared {
     float max;
     uint2 range[2];
     uint32_t upto_n[2], last_n[2];
-    uint2 upto[2][kList], last[2][kList];
+    uint2 upto[2][kList], last[2][kLast];
     unsigned long long sum[2];
     // this CTA's own
-    struct alignas(16) {
-        uint2 token;  // (index, key): in order as one number
-        unsigned long long weight;
-    } list[kList];
     unsigned long long before, target, total;
+    uint2 own[kWarps];
     int bucket;
     Border border;
     uint32_t flag;
 };
 
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    cluster_arrive();
+    cluster_wait();
 }
 __device__ __forceinline__ uint32_t peer_addr(const void *p, int rank) {
     uint32_t r;
@@ -199,36 +214,50 @@ __device__ __forceinline__ void each_near(const Row &row, float most, F f) {
 }
 __device__ __forceinline__ bool within(uint32_t key, uint32_t index, const Border &b) { return key < b.key || (key == b.key && index <= b.index); }
 
-// Adds up weights of tokens that are few among the warp's: they are gathered first, so that no lane computes a weight that does not count.
-struct Batch {
-    float *buf;  // of the warp: room for two spans
+// The warp's tokens that pass a cheap test, gathered until f can have four of them in every lane: f(logits, indices, which of the four there
+// are), called by all lanes.  What follows for a token that counts (keys, lists, 64-bit weights) takes ten times the test's instructions.
+struct Gather {
+    float *logit;  // of the warp: room for two spans
+    uint16_t *place;
     int waiting = 0;
-    unsigned long long sum = 0;  // of the lane
-    __device__ __forceinline__ Batch(Shared &s) : buf(s.batch[threadIdx.x >> 5]) {}
-    __device__ __forceinline__ void add(const Row &row, const float (&l)[4], const bool (&take)[4]) {
+    __device__ __forceinline__ Gather(Shared &s) : logit(s.batch[threadIdx.x >> 5]), place(s.place[threadIdx.x >> 5]) {}
+    template <class F>
+    __device__ __forceinline__ void add(const Row &row, const float (&l)[4], int index, const bool (&take)[4], F f) {
         if (!__any_sync(0xffffffffu, take[0] || take[1] || take[2] || take[3])) return;
-        const int lane = threadIdx.x & 31;
+        const unsigned below = (1u << (threadIdx.x & 31)) - 1u;
+        int at = waiting;  // (a population count takes a warp eight cycles)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) at += __popc(__ballot_sync(0xffffffffu, take[j]) & below);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (take[j]) {
+                logit[at] = l[j];
+                place[at] = (uint16_t)(index + j - row.first);
+                ++at;
+            }
+        waiting = __shfl_sync(0xffffffffu, at, 31);
+        __syncwarp();
+        if (waiting >= kSpan) some(row, kSpan, f);
+    }
+    template <class F>
+    __device__ __forceinline__ void finish(const Row &row, F f) {
+        if (waiting > 0) some(row, waiting, f);
+    }
+    template <class F>
+    __device__ __forceinline__ void some(const Row &row, int n, F f) {  // the last n, at most a span
+        waiting -= n;
+        float l[4];
+        uint32_t index[4];
+        bool there[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const unsigned mask = __ballot_sync(0xffffffffu, take[j]);
-            if (take[j]) buf[waiting + __popc(mask & ((1u << lane) - 1u))] = l[j];
-            waiting += __popc(mask);
+            const int i = 32 * j + (threadIdx.x & 31);
+            there[j] = i < n;
+            l[j] = there[j] ? logit[waiting + i] : -INFINITY;
+            index[j] = (uint32_t)row.first + (there[j] ? place[waiting + i] : 0u);
         }
         __syncwarp();
-        if (waiting < kSpan) return;
-        waiting -= kSpan;
-        const float4 v = *reinterpret_cast<const float4 *>(buf + 4 * lane);
-        sum += row.weight(v.x) + row.weight(v.y) + row.weight(v.z) + row.weight(v.w);
-        const float rest[4] = {buf[kSpan + lane], buf[kSpan + 32 + lane], buf[kSpan + 64 + lane], buf[kSpan + 96 + lane]};
-        __syncwarp();
-#pragma unroll
-        for (int j = 0; j < 4; ++j) buf[32 * j + lane] = rest[j];
-        __syncwarp();
-    }
-    __device__ __forceinline__ void finish(const Row &row) {
-        for (int i = threadIdx.x & 31; i < waiting; i += 32) sum += row.weight(buf[i]);
-        waiting = 0;
-        __syncwarp();
+        f(l, index, there);
     }
 };
 
@@ -356,18 +385,37 @@ __device__ __forceinline__ void clear_histogram(Shared &s, bool weights, bool &u
     __syncthreads();
 }
 
-// The cluster's lists (of up to kList tokens in all) as one, with weights: s.list.  A warp per CTA that has one.
-__device__ __forceinline__ void collect(Shared &s, const Row &row, const uint32_t *n_of, const uint2 *of) {
+// The cluster's lists (of up to kLast tokens in all) as one: s.list.  A warp per CTA that has one; n: how many the lane's has.
+template <bool WEIGHTS>
+__device__ __forceinline__ void collect(Shared &s, const Row &row, uint32_t n, const uint2 *of) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t n = lane < row.ctas ? peer_u32(n_of, lane) : 0u;
     const uint32_t at = __reduce_add_sync(0xffffffffu, lane < warp ? n : 0u), mine = __shfl_sync(0xffffffffu, n, warp);
     if (warp < row.ctas)
         for (uint32_t i = lane; i < mine; i += 32) {
             const unsigned long long e = peer_u64(of + i, warp);
             s.list[at + i].token = make_uint2((uint32_t)(e >> 32), (uint32_t)e);
-            s.list[at + i].weight = row.counts(logit_of((uint32_t)e)) ? Row::whole(row.units(logit_of((uint32_t)e))) : 0ull;
+            if constexpr (WEIGHTS) s.list[at + i].weight = row.counts(logit_of((uint32_t)e)) ? Row::whole(row.units(logit_of((uint32_t)e))) : 0ull;
         }
     __syncthreads();
+}
+// One value per thread of the first n to rising order (bitonic; those behind bring the largest value).  Warps behind all n only keep step.
+__device__ __forceinline__ unsigned long long sort_threads(Shared &s, unsigned long long v, uint32_t n) {
+    int turn = 0;
+    const bool busy = (threadIdx.x & ~31u) < n || (threadIdx.x & ~31u) < (1u << (32 - __clz(n - 1)));
+    auto step = [&](unsigned size, unsigned stride, unsigned long long other) {
+        return (((threadIdx.x & size) == 0) == ((threadIdx.x & stride) == 0)) == (other < v) ? other : v;
+    };
+    for (unsigned size = 2; size < 2 * n; size <<= 1) {
+        for (unsigned stride = size >> 1; stride >= 32; stride >>= 1) {
+            if (busy) s.exchange[turn][threadIdx.x] = v;
+            __syncthreads();
+            if (busy) v = step(size, stride, s.exchange[turn][threadIdx.x ^ stride]);
+            turn ^= 1;
+        }
+        if (busy)
+            for (unsigned stride = min(size >> 1, 16u); stride > 0; stride >>= 1) v = step(size, stride, __shfl_xor_sync(0xffffffffu, v, stride));
+    }
+    return v;
 }
 // How many of the list's tokens come before the thread's own (list[threadIdx.x % kList]), and their weights; two threads share a token, and
 // the second half's answer is no use
@@ -448,6 +496,7 @@ __device__ Selected find_border(Shared &s, const Row &row, const Goal &goal, con
     // the largest depths that round to the bucket, and to the one in front of it
     const float most = (bucket & 1) ? __uint_as_float(__float_as_uint((float)bucket + 0.5f) - 1u) : (float)bucket + 0.5f;
     const float most_front = bucket == 0 ? -1.0f : (bucket & 1) ? (float)bucket - 0.5f : __uint_as_float(__float_as_uint((float)bucket - 0.5f) - 1u);
+    const int lane = threadIdx.x & 31;
     bool ranged = false, ranked = false;
     for (;;) {
         // ---- the tokens that are left (and, the first time, all in front of them), if they are few ----
@@ -455,68 +504,88 @@ __device__ Selected find_border(Shared &s, const Row &row, const Goal &goal, con
         ++turn;
         if (threadIdx.x == 0) s.upto_n[h] = s.last_n[h] = 0;
         __syncthreads();
-        bool open = !ranged;  // while the longer list has room
-        Batch front(s);       // tokens of the buckets in front
+        // while the longer list has room; counted tokens in front say beforehand whether it has
+        const bool all_few = !ranged && (goal.by_weight || before < kList);
+        bool open = all_few;
+        unsigned long long front = 0;  // weights of tokens in the buckets in front
+        auto look = [&](const float (&l)[4], const uint32_t (&index)[4], const bool (&there)[4]) {
+            unsigned here[4], ahead[4];
+            uint32_t key[4], n_here = 0, n_ahead = 0;
+            unsigned long long w[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[j] = final && !ranged ? row.weight(l[j]) : 0ull;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const bool in_front = row.depth(l[j]) <= most_front, in = there[j] && inside(l[j], index[j]);
+                key[j] = key_of(l[j]);
+                here[j] = __ballot_sync(0xffffffffu, in && !in_front && key[j] >= lo && key[j] <= hi);
+                ahead[j] = __ballot_sync(0xffffffffu, in && in_front);
+                n_here += __popc(here[j]);
+                n_ahead += __popc(ahead[j]);
+                front += in && in_front ? w[j] : 0ull;
+            }
+            auto append = [&](uint32_t &count, uint2 *list, uint32_t most, uint32_t n, auto mask) {  // a place for the warp's tokens at once
+                uint32_t at = 0;
+                if (lane == 0) at = atomicAdd(&count, n);
+                at = __shfl_sync(0xffffffffu, at, 0);
+                const bool room = at + n <= most;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const unsigned m = mask(j);
+                    const uint32_t place = at + __popc(m & ((1u << lane) - 1u));
+                    if ((m >> lane & 1u) && place < most) list[place] = make_uint2(key[j], index[j]);
+                    at += __popc(m);
+                }
+                return room;
+            };
+            if (n_here) append(s.last_n[h], s.last[h], kLast, n_here, [&](int j) { return here[j]; });
+            if (open) open = append(s.upto_n[h], s.upto[h], kList, n_here + n_ahead, [&](int j) { return here[j] | ahead[j]; });
+        };
+        Gather near(s);
         each_span(row, [&](const float (&l)[4], int index) {
-            bool here[4], ahead[4];
-            open = open && *reinterpret_cast<volatile uint32_t *>(&s.upto_n[h]) <= kList;
-            bool any = false;
+            bool take[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const float d = row.depth(l[j]);
-                const bool in = d <= most && inside(l[j], (uint32_t)(index + j));
-                ahead[j] = in && d <= most_front;
-                here[j] = in && !ahead[j];
-                any = any || here[j] || (open && ahead[j]);
+                take[j] = d <= most && (d > most_front || open || (final && !ranged));
             }
-            if (any) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const uint2 e = make_uint2(key_of(l[j]), (uint32_t)(index + j));
-                    if (here[j] && e.x >= lo && e.x <= hi) {
-                        const uint32_t at = atomicAdd(&s.last_n[h], 1u);
-                        if (at < kList) s.last[h][at] = e;
-                    }
-                    if (open && (here[j] || ahead[j])) {
-                        const uint32_t at = atomicAdd(&s.upto_n[h], 1u);
-                        if (at < kList) s.upto[h][at] = e;
-                    }
-                }
-            }
-            if (final && !ranged) front.add(row, l, ahead);
+            near.add(row, l, index, take, look);
         });
-        if (final && !ranged) {
-            front.finish(row);
-            sum = front.sum;
-        }
+        near.finish(row, look);
+        if (final && !ranged) sum = front;
         cluster_sync();
-        const int lane = threadIdx.x & 31;
-        const uint32_t upto_n = __reduce_add_sync(0xffffffffu, lane < row.ctas ? peer_u32(&s.upto_n[h], lane) : 0u);
-        const uint32_t last_n = __reduce_add_sync(0xffffffffu, lane < row.ctas ? peer_u32(&s.last_n[h], lane) : 0u);
-        if (!ranged && upto_n <= kList) {
-            if (row.rank == 0) collect(s, row, &s.upto_n[h], s.upto[h]);
+        const uint32_t upto_of = lane < row.ctas ? peer_u32(&s.upto_n[h], lane) : 0u, last_of = lane < row.ctas ? peer_u32(&s.last_n[h], lane) : 0u;
+        const uint32_t upto_n = __reduce_add_sync(0xffffffffu, upto_of), last_n = __reduce_add_sync(0xffffffffu, last_of);
+        if (all_few && upto_n <= kList) {
+            if (row.rank == 0) collect<true>(s, row, upto_of, s.upto[h]);
             listed = upto_n;
             return kListed;
         }
-        if (last_n <= kList) {
-            collect(s, row, &s.last_n[h], s.last[h]);
-            unsigned long long in_front;
-            const uint32_t rank = rank_in_list(s, last_n, in_front);
-            if (threadIdx.x < last_n) {
-                const uint2 me = s.list[threadIdx.x].token;
-                const unsigned long long from = before + (goal.by_weight ? in_front : rank);
-                if (from < s.target && s.target <= from + (goal.by_weight ? s.list[threadIdx.x].weight : 1ull)) s.border = {me.y, me.x};
-            }
+        if (last_n <= kLast) {
+            if (threadIdx.x < kWarps) s.own[threadIdx.x] = make_uint2(0u, 0u);
+            collect<false>(s, row, last_of, s.last[h]);
+            auto order = [](uint2 t) { return ((unsigned long long)t.y << 32) | t.x; };
+            const bool has = threadIdx.x < last_n;
+            const unsigned long long me = sort_threads(s, has ? order(s.list[threadIdx.x].token) : ~0ull, last_n);
+            const uint32_t key = (uint32_t)(me >> 32), index = (uint32_t)me;
+            const float l = logit_of(key);
+            const double units = row.units(l);
+            const unsigned long long w = has && row.counts(l) ? Row::whole(units) : 0ull, mine = goal.by_weight ? w : has ? 1ull : 0ull;
+            unsigned long long from, all;
+            block_scan(s, mine, from, all);
+            from += before;
+            if (from < s.target && s.target <= from + mine) s.border = {key, index};
             __syncthreads();
             border = s.border;
             if (!final) return kBorder;
-            if (!ranged) {  // the warp's own of the list, up to the border
-                const int own = row.first + (int)(threadIdx.x >> 5) * row.share;
-                const uint32_t begin = (uint32_t)max(own, row.begin), end = (uint32_t)min(own + row.share, row.end);
-                for (uint32_t i = lane; i < last_n; i += 32) {
-                    const uint2 e = s.list[i].token;
-                    if (e.x >= begin && e.x < end && within(e.y, e.x, border)) sum += row.weight(logit_of(e.y));
+            if (!ranged) {  // the warps' own of the list, up to the border, in two pieces
+                const uint32_t at = index - (uint32_t)row.first;
+                if (has && index >= (uint32_t)row.begin && index < (uint32_t)row.end && within(key, index, border) && (units >= row.least || l == row.max)) {
+                    atomicAdd(&s.own[at / (uint32_t)row.share].x, (uint32_t)w & 0x3fffffu);
+                    atomicAdd(&s.own[at / (uint32_t)row.share].y, (uint32_t)(w >> 22));
                 }
+                __syncthreads();
+                if (lane == 0) sum += s.own[threadIdx.x >> 5].x + ((unsigned long long)s.own[threadIdx.x >> 5].y << 22);
                 return kBorder;
             }
             ranked = true;
@@ -588,7 +657,6 @@ __device__ Selected find_border(Shared &s, const Row &row, const Goal &goal, con
         const uint32_t key = key_of(v);
         if (key == lo && candidate(v, key, index)) ++mine;
     });
-    const int lane = threadIdx.x & 31;
     mine = __reduce_add_sync(0xffffffffu, mine);  // of the warp, whose tokens are neighbours
     unsigned long long ahead, total;
     block_scan(s, lane == 0 ? mine : 0u, ahead, total);
@@ -834,15 +902,18 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
             each_near(row, 0.0f, [&](float l, uint32_t) { mine += l == row.max ? 1ull : 0ull; });
         } else if (limited) {
             mine = 0;
-            Batch kept(s);
+            auto add = [&](const float (&l)[4], const uint32_t (&)[4], const bool (&there)[4]) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) mine += there[j] ? row.weight(l[j]) : 0ull;
+            };
+            Gather kept(s);
             each_span(row, [&](const float (&l)[4], int index) {
                 bool take[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) take[j] = within(key_of(l[j]), (uint32_t)(index + j), limit);
-                kept.add(row, l, take);
+                kept.add(row, l, index, take, add);
             });
-            kept.finish(row);
-            mine = kept.sum;
+            kept.finish(row, add);
         } else {
             mine = 0;
             each_span(row, [&](const float (&l)[4], int) {
@@ -866,6 +937,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
         if (q < row.rank) ahead += t;
         all += t;
     }
+    __syncthreads();
+    cluster_arrive();  // this CTA reads the others' memory no more
     if (all == 0) {  // nothing above -inf
         if (row.rank == 0 && threadIdx.x == 0) {
             p.ids[b] = -1;
@@ -912,7 +985,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
             }
         }
     }
-    cluster_sync();  // the others may still read this CTA's memory
+    cluster_wait();  // nor they this one's
 }
 
 struct SmemOnce {

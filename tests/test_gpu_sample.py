@@ -264,3 +264,25 @@ def test_least_temperature(dev):
 
     ids, probs = lb.sample(logits.to(dev), torch.from_numpy(u.astype(np.float32)).to(dev), temperature=2.0 ** -121)
     assert ids.tolist() == [1, 1, 1] and probs.tolist() == [1.0, 1.0, 1.0]
+
+
+@pytest.mark.parametrize("n", [1, 2, 33, 64, 65, 200, 257, 511, 512, 513, 700])
+def test_tokens_of_one_bucket(dev, n):
+    """The border among n tokens that lie within 1/64 of one another, behind 300 others: sorted, or searched by ranges; for weights and for counts."""
+    rng = np.random.default_rng(n)
+    v = 300 + n + 20000
+    rows = []
+    for ties in (False, True):
+        near = 2.0 + rng.random(n) * 0.006
+        if ties:
+            near = 2.0 + rng.integers(0, 3, n) * 0.002
+        row = np.concatenate([4 + rng.random(300), near, -6 - rng.random(20000)])
+        rows.append(row[rng.permutation(v)])
+    logits = torch.from_numpy(np.array(rows).astype(np.float32))
+    w = np.exp(np.sort(logits.double().numpy(), 1)[:, ::-1] - logits.double().max(1).values.numpy()[:, None])
+    u = np.array([0.999, 0.97])
+    for share in (0.1, 0.5, 0.93):
+        at = 300 + int(share * n)
+        check(dev, logits, u, k=at + 1)
+        check(dev, logits, u, p=(w[:, :at].sum(1) + 0.5 * w[:, at]) / w.sum(1))
+        check(dev, logits, u, k=at + 1, p=0.9999, mp=1e-6)

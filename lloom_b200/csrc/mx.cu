@@ -300,6 +300,12 @@ __device__ __forceinline__ void put4(__nv_bfloat16 *y, const float4 &v) {
     *reinterpret_cast<uint2 *>(y) = make_uint2(*reinterpret_cast<const uint32_t *>(&a), *reinterpret_cast<const uint32_t *>(&b));
 }
 
+// After a wait that ran out: the copies that a thread has started, `issued` stages in turn, end or run out of time themselves
+__device__ __forceinline__ void drain(uint64_t *full, int issued, int stages) {
+    for (int i = max(issued - stages, 0); i < issued; ++i)
+        if (!mbar_wait(&full[i % stages], (uint32_t)(i / stages) & 1u)) break;
+}
+
 // One 128 x bn tile per cluster; its CTAs take equal parts of K, and the parts' sums meet in shared memory in a fixed order.
 // QUANTIZE: up to sixteen activation rows, which every CTA quantizes itself, its part of K, while the first weights are on their way: one launch
 // instead of two.
@@ -320,6 +326,7 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx_gemm_kernel(const __grid_con
     const int count = u1 - u0;
     constexpr int kABytes = mx_unit_bytes(kMxTile), kQuantUnit = mx_unit_bytes(16);
     const int b_bytes = QUANTIZE ? 0 : mx_unit_bytes(p.bn);
+    int issued = 0;  // stages that this thread has started to fill
 
     launch_dependents();
     if (threadIdx.x == 0) {
@@ -341,6 +348,7 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx_gemm_kernel(const __grid_con
                 mbar_arrive_expect_tx(&full[i], (uint32_t)(kABytes + b_bytes));
                 bulk_g2s(ring + i * p.stage_bytes, w + (int64_t)i * kABytes, kABytes, &full[i]);
             }
+            issued = first;
             wait_predecessor();  // the activation image is there
             if (!QUANTIZE)
                 for (int i = 0; i < first; ++i) bulk_g2s(ring + i * p.stage_bytes + kABytes, a + (int64_t)i * b_bytes, (uint32_t)b_bytes, &full[i]);
@@ -351,6 +359,7 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx_gemm_kernel(const __grid_con
                 mbar_arrive_expect_tx(&full[s], (uint32_t)(kABytes + b_bytes));
                 bulk_g2s(ring + s * p.stage_bytes, w + (int64_t)i * kABytes, kABytes, &full[s]);
                 if (!QUANTIZE) bulk_g2s(ring + s * p.stage_bytes + kABytes, a + (int64_t)i * b_bytes, (uint32_t)b_bytes, &full[s]);
+                ++issued;
                 if (++s == p.stages) {
                     s = 0;
                     par ^= 1;
@@ -446,6 +455,11 @@ __global__ void __launch_bounds__(kMxThreads, 1) mx_gemm_kernel(const __grid_con
     }
     tc_fence_before();
     __syncthreads();
+    if (*abort_flag) {  // what is in flight ends first
+        if (warp == kMxQuantWarps && lane == 0) drain(full, issued, p.stages);
+        if (warp == kMxQuantWarps + 1) mbar_wait(done, 0);
+        __syncthreads();
+    }
     if (warp == kMxQuantWarps + 1) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(*tmem_slot), "r"((uint32_t)p.tmem_cols));
@@ -563,8 +577,8 @@ __global__ void __launch_bounds__(kPairThreads, 1) mx_gemm_pair_kernel(const __g
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     uint64_t *full = reinterpret_cast<uint64_t *>(smem + p.stages * p.stage_bytes), *empty = full + kPairStages;
-    uint64_t *acc_full = empty + kPairStages, *acc_empty = acc_full + 2;
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(acc_empty + 2);
+    uint64_t *acc_full = empty + kPairStages, *acc_empty = acc_full + 2, *drained = acc_empty + 2;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drained + 1);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -572,6 +586,8 @@ __global__ void __launch_bounds__(kPairThreads, 1) mx_gemm_pair_kernel(const __g
     const int tiles = (p.n_tiles + 1) / 2 * p.m_tiles, first = blockIdx.x >> 1, step = gridDim.x >> 1;
     constexpr int kABytes = mx_unit_bytes(kMxTile);
     const int half = p.bn / 2 * 128, part_bytes = half + mx_scale_bytes(p.bn), part_rows = part_bytes / 128;
+    int issued = 0;
+    bool issuer = false;
 
     launch_dependents();
     if (threadIdx.x == 0) {
@@ -583,6 +599,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) mx_gemm_pair_kernel(const __g
             mbar_init(&acc_full[i], 1);
             mbar_init(&acc_empty[i], 2 * kPairEpiWarps);
         }
+        mbar_init(drained, 1);
         *abort_flag = 0;
         fence_mbar_init();
     }
@@ -621,6 +638,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) mx_gemm_pair_kernel(const __g
                     if (rank == 0) mbar_arrive_expect_tx(&full[s], (uint32_t)(2 * (kABytes + part_bytes)));
                     copy_rows(dst, &p.w, w, bar);
                     copy_rows(dst + kABytes, &p.a, a, bar);
+                    ++issued;
                     w += kABytes / 128;
                     a += 2 * part_rows;
                     if (++s == p.stages) {
@@ -633,7 +651,8 @@ __global__ void __launch_bounds__(kPairThreads, 1) mx_gemm_pair_kernel(const __g
         __syncwarp();
     } else if (warp == kPairEpiWarps + 1) {
         // ---- MMA, for both CTAs ----
-        if (rank == 0 && elect_one()) {
+        issuer = rank == 0 && elect_one();
+        if (issuer) {
             const int groups = (p.bn + 127) / 128;
             const uint32_t sfa = tmem + 2 * (uint32_t)p.bn, sfb = sfa + 8;
             const uint32_t idesc = (1u << 7) | (1u << 10) | ((uint32_t)(p.bn >> 3) << 17) | (1u << 23) | (2u << 27);
@@ -718,6 +737,16 @@ __global__ void __launch_bounds__(kPairThreads, 1) mx_gemm_pair_kernel(const __g
     }
     tc_fence_before();
     __syncthreads();
+    if (*abort_flag) {  // what is in flight ends first; the second CTA's copies, which arrive at the first one's barriers, have a millisecond
+        if (rank == 0 && warp == kPairEpiWarps && lane == 0) drain(full, issued, p.stages);
+        if (issuer) {
+            umma2_commit(drained);
+            mbar_wait(drained, 0);
+        }
+        if (rank == 1 && warp == kPairEpiWarps)
+            for (int i = 0; i < 1000; ++i) __nanosleep(1000);
+        __syncthreads();
+    }
     cluster_arrive();
     cluster_wait();  // neither reads the other's memory, or computes into it, any more
     if (warp == kPairEpiWarps + 1) {

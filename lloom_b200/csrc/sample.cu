@@ -16,8 +16,8 @@
 // exp: table of 2^(-j/32) and a polynomial (table-driven, after Tang 1989) in 64-bit arithmetic, relative error below 5e-14.
 //
 // Bound by latency for a few rows: a launch, one read of DRAM, six to eight cluster barriers of about a microsecond with short passes between
-// them (1 x 128256 f32 with all filters 15.5 us, 7 x 50257 bf16 with top-p 33).  For many rows by the passes themselves: shared-memory
-// additions (nine cycles each) and 64-bit arithmetic (two cycles a warp and multiply-add) of the weights: 64 x 128256 f32, 33 MB, settings of their own, 71 us.
+// them (1 x 128256 f32 with all filters 15.3 us, 7 x 50257 bf16 with top-p 33).  For many rows by the passes themselves: shared-memory
+// additions (nine cycles each) and 64-bit arithmetic (two cycles a warp and multiply-add) of the weights: 64 x 128256 f32, 33 MB, settings of their own, 68 us.
 // There a row read from L2 in every pass by fewer CTAs, all rows at once, was faster for alike rows (75 us for 85) and slower for unlike ones (126 for 84).
 #include <mutex>
 #include <type_traits>
@@ -84,7 +84,7 @@ struct Shared {
     // read by the other CTAs too; two of each, used in turn: what one exchange leaves is rewritten only behind the barrier of the next
     float max;
     uint2 range[2];
-    uint32_t upto_n[2], last_n[2];
+    uint32_t listed[2], last_n[2];  // listed: lengths of the lists, of `last` in the upper half (a CTA has fewer than 2^16 tokens)
     uint2 upto[2][kList], last[2][kLast];
     unsigned long long sum[2];
     // this CTA's own
@@ -502,7 +502,7 @@ __device__ Selected find_border(Shared &s, const Row &row, const Goal &goal, con
         // ---- the tokens that are left (and, the first time, all in front of them), if they are few ----
         const int h = turn & 1;
         ++turn;
-        if (threadIdx.x == 0) s.upto_n[h] = s.last_n[h] = 0;
+        if (threadIdx.x == 0) s.listed[h] = 0;
         __syncthreads();
         // while the longer list has room; counted tokens in front say beforehand whether it has
         const bool all_few = !ranged && (goal.by_weight || before < kList);
@@ -524,22 +524,24 @@ __device__ Selected find_border(Shared &s, const Row &row, const Goal &goal, con
                 n_ahead += __popc(ahead[j]);
                 front += in && in_front ? w[j] : 0ull;
             }
-            auto append = [&](uint32_t &count, uint2 *list, uint32_t most, uint32_t n, auto mask) {  // a place for the warp's tokens at once
-                uint32_t at = 0;
-                if (lane == 0) at = atomicAdd(&count, n);
-                at = __shfl_sync(0xffffffffu, at, 0);
-                const bool room = at + n <= most;
+            // places for the warp's tokens at once
+            const uint32_t n_upto = open ? n_here + n_ahead : 0u, n = n_here << 16 | n_upto;
+            if (n == 0) return;
+            uint32_t at = 0;
+            if (lane == 0) at = atomicAdd(&s.listed[h], n);
+            at = __shfl_sync(0xffffffffu, at, 0);
+            uint32_t last = at >> 16, upto = at & 0xffffu;
+            open = open && upto + n_upto <= kList;
+            const unsigned below = (1u << lane) - 1u;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const unsigned m = mask(j);
-                    const uint32_t place = at + __popc(m & ((1u << lane) - 1u));
-                    if ((m >> lane & 1u) && place < most) list[place] = make_uint2(key[j], index[j]);
-                    at += __popc(m);
-                }
-                return room;
-            };
-            if (n_here) append(s.last_n[h], s.last[h], kLast, n_here, [&](int j) { return here[j]; });
-            if (open) open = append(s.upto_n[h], s.upto[h], kList, n_here + n_ahead, [&](int j) { return here[j] | ahead[j]; });
+            for (int j = 0; j < 4; ++j) {
+                const unsigned all = here[j] | ahead[j];
+                const uint32_t to_last = last + __popc(here[j] & below), to_upto = upto + __popc(all & below);
+                if ((here[j] >> lane & 1u) && to_last < kLast) s.last[h][to_last] = make_uint2(key[j], index[j]);
+                if (n_upto && (all >> lane & 1u) && to_upto < kList) s.upto[h][to_upto] = make_uint2(key[j], index[j]);
+                last += __popc(here[j]);
+                upto += __popc(all);
+            }
         };
         Gather near(s);
         each_span(row, [&](const float (&l)[4], int index) {
@@ -554,7 +556,7 @@ __device__ Selected find_border(Shared &s, const Row &row, const Goal &goal, con
         near.finish(row, look);
         if (final && !ranged) sum = front;
         cluster_sync();
-        const uint32_t upto_of = lane < row.ctas ? peer_u32(&s.upto_n[h], lane) : 0u, last_of = lane < row.ctas ? peer_u32(&s.last_n[h], lane) : 0u;
+        const uint32_t of = lane < row.ctas ? peer_u32(&s.listed[h], lane) : 0u, upto_of = of & 0xffffu, last_of = of >> 16;
         const uint32_t upto_n = __reduce_add_sync(0xffffffffu, upto_of), last_n = __reduce_add_sync(0xffffffffu, last_of);
         if (all_few && upto_n <= kList) {
             if (row.rank == 0) collect<true>(s, row, upto_of, s.upto[h]);

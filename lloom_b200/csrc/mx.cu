@@ -17,7 +17,8 @@
 //
 // Bound by: one row of small matrices, the latency of one launch and a chain of copy, products, reduction ([1024, 4096] 4.3 us); a few rows of large
 // ones, reading the weights (8 x [14336, 4096] 7.2 us, 31 MB: 4.3 TB/s with all of start and end); many rows, the tensor cores and
-// what L2 gives an SM (2048 x [14336, 4096] 73 us from new inputs: 3.3 PFLOP/s; 512 x [4096, 14336] 26 us: 2.3).  Quantizing 512 x 4096 bf16 takes
+// what L2 gives an SM (2048 x [14336, 4096] 51 us, 4.7 PFLOP/s, the tensor pipe 75 % busy; 73 with the quantizer and from new inputs; 512 x [4096, 14336]
+// 26 us: 2.3).  Quantizing 512 x 4096 bf16 takes
 // 2.4 us, reading the values back as f32 4.3.
 #include <algorithm>
 #include <mutex>

@@ -320,3 +320,33 @@ def test_plans_agree(dev):
         want = (x.double() @ w.double().T).float()
         for m in (1, 2, 4, 16, 17, 65, 128, 129, 250, 384, 520):
             assert torch.equal(mm.forward(x[:m].to(dev)).cpu(), want[:m]), (n, k, m)
+
+
+@pytest.mark.parametrize("m,n,k", [(70001, 3, 32), (33000, 130, 96), (1, 70001, 32), (300, 40001, 64)])
+def test_many_rows(dev, m, n, k):
+    """More rows than a grid's second dimension has, on either side."""
+    from lloom_b200 import MxMatMul, MxTensor
+
+    w, x = whole(1, n, k), whole(2, m, k)
+    t = MxTensor.quantize(w.to(dev))
+    assert torch.equal(t.dequantize().cpu(), w)
+    got = MxMatMul.from_tensor(t).forward(x.to(dev))
+    assert torch.equal(got.double(), x.to(dev).double() @ w.to(dev).double().T)
+    assert torch.equal(MxTensor.quantize(x.to(dev)).dequantize().cpu(), x)
+    again = MxTensor.from_data(t.data(), (n, k), dev)
+    assert torch.equal(again.dequantize().cpu(), w)
+
+
+@pytest.mark.parametrize("m,n,k", [(33000, 66000, 32), (40, 1100000, 4096)])
+def test_offsets_past_32_bits(dev, m, n, k):
+    """More than 2^31 outputs; an image of more than 2^31 bytes: rows that repeat, at the end as at the beginning."""
+    from lloom_b200 import MxMatMul, MxTensor
+
+    w, x = whole(1, 100, k), whole(2, 40, k)
+    mm = MxMatMul.from_tensor(MxTensor.quantize(w.to(dev).bfloat16().repeat(n // 100, 1)))
+    y = mm.forward(x.to(dev).bfloat16().repeat(m // 40, 1))
+    want = (x.double() @ w.double().T).bfloat16().to(dev)
+    for rows in (slice(0, 40), slice(m - 40, m)):
+        for cols in (slice(0, 100), slice(n - 100, n)):
+            assert torch.equal(y[rows, cols], want)
+    assert (y.view(m // 40, -1)[:: max(1, m // 400)] == y[:40].reshape(-1)).all()

@@ -267,3 +267,38 @@ def test_many_rows(dev, m, k, x):
     z[0, 3:], z[1, 3:] = a.view(-1).to(dev), r.view(-1).to(dev)
     y2, h2 = rms_norm(z[0, 3:].view(m, k), w.to(dev), EPS, z[1, 3:].view(m, k))
     assert torch.equal(y, y2) and torch.equal(h, h2)
+
+
+@pytest.mark.parametrize("m,k,act", [(70001, 32, "Q8_0"), (70001, 256, "Q4K"), (140003, 9, None), (70001, 520, None)])
+def test_rows_past_a_grid(dev, m, k, act):
+    """More than 65535 rows, rows that share a CTA among them; as in two halves."""
+    import lloom_b200 as lb
+
+    a, r, w = (t.to(dev) for t in inputs(m + k, m, k, torch.bfloat16))
+    kind = None if act is None else getattr(lb.GgmlDType, act)
+    y, h = lb.rms_norm(a, w, EPS, r, act_for=kind)
+    cut = m // 2
+    parts = [lb.rms_norm(a[s], w, EPS, r[s], act_for=kind) for s in (slice(0, cut), slice(cut, m))]
+    assert torch.equal(h, torch.cat([p[1] for p in parts])) and torch.equal(h, (a.float() + r.float()).bfloat16())
+    if act is None:
+        assert torch.equal(y, torch.cat([p[0] for p in parts]))
+    else:
+        assert torch.equal(y.blocks, torch.cat([p[0].blocks for p in parts]))
+        assert torch.equal(y.dequantize(), torch.cat([p[0].dequantize() for p in parts]))
+
+
+@pytest.mark.parametrize("act", [None, "Q4K"])
+def test_offsets_past_32_bits(dev, act):
+    """A stream of more than 2^31 elements: its last rows as its first ones."""
+    import lloom_b200 as lb
+
+    a, r, w = (t.to(dev) for t in inputs(5, 64, 16384, torch.bfloat16))
+    reps = 2 ** 31 // (64 * 16384) + 1
+    kind = None if act is None else getattr(lb.GgmlDType, act)
+    y, h = lb.rms_norm(a.repeat(reps, 1), w, EPS, r.repeat(reps, 1), act_for=kind)
+    y1, h1 = lb.rms_norm(a, w, EPS, r, act_for=kind)
+    if act is not None:
+        y, y1 = y.blocks, y1.blocks
+    for got, want in ((y, y1), (h, h1)):
+        assert torch.equal(got[:64], want) and torch.equal(got[-64:], want)
+        assert (got.view(reps, 64, -1)[::97] == want).all()

@@ -286,3 +286,35 @@ def test_tokens_of_one_bucket(dev, n):
         check(dev, logits, u, k=at + 1)
         check(dev, logits, u, p=(w[:, :at].sum(1) + 0.5 * w[:, at]) / w.sum(1))
         check(dev, logits, u, k=at + 1, p=0.9999, mp=1e-6)
+
+
+@pytest.mark.parametrize("b,v", [(70001, 5), (3000, 517), (300, 9000)])
+def test_more_rows_than_fit_at_once(dev, b, v):
+    """Settings of their own for every row; rows that repeat give the same token."""
+    import lloom_b200 as lb
+
+    base, u = rand(b, 50, v)
+    reps = -(-b // 50)
+    logits, u = base.repeat(reps, 1)[:b], np.tile(u, reps)[:b]
+    t = np.tile(np.linspace(0.0, 2.0, 50, dtype=np.float32), reps)[:b]
+    k = np.tile(np.arange(50, dtype=np.int32), reps)[:b]
+    p = np.tile(np.linspace(0.3, 1.0, 50, dtype=np.float32), reps)[:b]
+    check(dev, logits[:50], u[:50], t=t[:50], k=k[:50], p=p[:50])
+    args = [torch.from_numpy(a).to(dev) for a in (u, t, k, p)]
+    ids, probs = lb.sample(logits.to(dev), *args)
+    for out in (ids, probs):
+        full = torch.cat([out, out[-50:]])
+        assert torch.equal(out[50:], out[:-50]) and full.shape[0] == b + 50
+
+
+def test_logits_past_32_bits(dev):
+    """A batch of more than 2^31 logits: its last rows as its first ones."""
+    import lloom_b200 as lb
+
+    base, u = rand(1, 8, 50257, torch.float16)
+    reps = 2 ** 31 // (8 * 50257) + 2
+    logits = base.to(dev).repeat(reps, 1)
+    assert logits.numel() > 2 ** 31
+    ids, probs = lb.sample(logits, torch.from_numpy(u).to(dev).repeat(reps), top_p=0.8)
+    assert (ids.view(reps, 8) == ids[:8]).all() and (probs.view(reps, 8) == probs[:8]).all()
+    check(dev, base, u, p=0.8)

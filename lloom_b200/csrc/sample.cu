@@ -1030,11 +1030,18 @@ int sample(const void *logits, int type, int64_t batch, int64_t vocab, int64_t l
     p.min_p_all = min_p_all;
     p.ids = ids;
     p.probs = probs;
+    // CTAs to a row: up to eight with more than 2048 logits each; half as many while there are more CTAs than SMs and a part of the row twice as
+    // long still leaves room for another CTA on the SM: half of a CTA's work does not depend on how many logits it has.  us by 8 / 4 / 2 / 1 CTAs:
+    // 7 x 50257 31 / 35 / 46; 19 x 128256 40 / 46; 19 x 32000 31 / 26 / 31 / 42; 30 x 50257 35 / 31 / 37; 37 x 50257 54 / 40 / 37; 64 x 32000 55 / 36 / 34 / 42; 64 x 128256 85 / 79 (alike rows; others level);
+    // 300 x 8000 179 / 87 / 52 / 42; 1000 x 32000 673 / 353 / 232 / 239.
+    auto share = [&](int ctas) { return (((vocab + ctas - 1) / ctas + 3 + kWarps - 1) / kWarps + kSpan - 1) / kSpan * kSpan; };
+    auto bytes = [&](int ctas) { return (int64_t)((sizeof(Shared) + 15) / 16 * 16) + kBuckets / ctas * 8 + kWarps * share(ctas) * 4; };
     int ctas = 1;
     while (ctas < kMaxCluster && vocab > (int64_t)ctas * 4096) ctas *= 2;
+    while (ctas > 1 && batch * ctas > di.sm_count && 2 * (bytes(ctas / 2) + di.smem_reserved) <= di.smem_per_sm) ctas /= 2;
     p.chunk = (int)((vocab + ctas - 1) / ctas);
-    p.share = ((p.chunk + 3 + kWarps - 1) / kWarps + kSpan - 1) / kSpan * kSpan;
-    const int smem = (int)((sizeof(Shared) + 15) / 16 * 16) + kBuckets / ctas * 8 + kWarps * p.share * 4;
+    p.share = (int)share(ctas);
+    const int smem = (int)bytes(ctas);
     static SmemOnce once;
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);

@@ -13,7 +13,8 @@
 // Weights are summed as integers, in units of 2^-43 of the largest weight: the sums are exact, so that they depend neither on
 // the split of a row nor on the order of atomics, and borders fall where 64-bit arithmetic puts them.  (In 32 bits a running sum over
 // 100,000 tokens is off by more than a token's share of it.)  Tokens below 2^-44 of the largest weight count as zero.
-// exp: table of 2^(-j/32) and a polynomial (table-driven, after Tang 1989) in 64-bit arithmetic, relative error below 5e-14.
+// exp in 64-bit arithmetic: the difference to the maximum times 1 / (T ln 2) is split into a whole number, the exponent, and the rest, a polynomial of
+// degree 9; relative error below 3e-14 at every temperature and size of the logits.
 //
 // Bound by latency for a few rows: a launch, one read of DRAM, six to eight cluster barriers of about a microsecond with short passes between
 // them (1 x 128256 f32 with all filters 15.3 us, 7 x 50257 bf16 with top-p 33).  For many rows by instruction issue and barriers
@@ -138,7 +139,7 @@ struct Row {
     unsigned long long *part;  // this CTA's, in shared memory: running sums of all histograms over its share of the buckets
     int ctas, rank;
     float max;            // finite
-    double at_max, slope; // at_max + slope * (the logit's bits as those of a double, in units of 2^-896) = (max - l) / T / ln 2
+    double wide_max, slope; // the maximum as widen() has it; slope * (wide_max - widen(l)) = (max - l) / T / ln 2
     float bucket_scale;   // 64 / T, finite
     double least;         // min_p in units of 2^-43
 
@@ -146,16 +147,20 @@ struct Row {
     // logits, so that a bucket is a range of them; 32 bits will do.
     __device__ __forceinline__ float depth(float l) const { return __fmul_rn(__fsub_rn(max, l), bucket_scale); }
     __device__ __forceinline__ int bucket(float l) const { return (int)(__float_as_uint(__fadd_rn(fminf(depth(l), (float)(kBuckets - 1)), 8388608.0f)) & 0x7fffffu); }
+    // l * 2^-896, exactly, subnormal ones too: its bits, moved to the places of a double's
+    static __device__ __forceinline__ double widen(float l) {
+        const uint32_t bits = __float_as_uint(l);
+        return __hiloint2double((int)(((int)bits >> 3) & 0x8fffffff), (int)(bits << 29));
+    }
     // exp(-(max - l) / T) in units of 2^-43, for tokens with `counts`: 2^-n by the exponent, 2^-z, |z| <= 1/2, by a polynomial fitted at
     // Chebyshev nodes (2e-14).  No conversions (eight cycles a warp; a multiply-add takes two) and no table (a random look-up in shared memory
-    // costs more than the five multiply-adds it would save): a logit is widened by moving its bits, whole numbers are read from sums
-    // with 1.5 * 2^52.
+    // costs more than the five multiply-adds it would save): whole numbers are read from sums with 1.5 * 2^52.
+    // The difference comes first, then the factor: for n + z = 46 at most (`counts`) the two roundings are off by 46 * 2^-52, whatever the logits'
+    // size, and the maximum's own weight is that of 0.  (Two products, of the maximum and of the logit, would each be rounded at the size of max / T.)
     __device__ __forceinline__ bool counts(float l) const { return depth(l) < (float)(kBuckets - 1) - 0.5f; }
     __device__ __forceinline__ double units(float l) const {
         constexpr double magic = 6755399441055744.0;
-        const uint32_t bits = __float_as_uint(l);
-        const double wide = __hiloint2double((int)(((int)bits >> 3) & 0x8fffffff), (int)(bits << 29));  // l * 2^-896
-        const double t = fma(wide, slope, at_max), m = t + magic, z = t - (m - magic);
+        const double below = wide_max - widen(l), m = fma(below, slope, magic), z = fma(below, slope, magic - m);
         double p = fma(z, -1.0205905407077635e-07 * kUnit, 1.3259645243921192e-06 * kUnit);
         p = fma(z, p, -1.5252672924891586e-05 * kUnit);
         p = fma(z, p, 0.00015403433751254647 * kUnit);
@@ -811,8 +816,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     const bool greedy = !(temperature >= kLeastTemperature);
     const double inv_t = greedy ? 0.0 : 1.0 / temperature;
     const double per_logit = inv_t * 1.4426950408889634074;  // 1 / ln 2 / T
-    row.at_max = (double)top * per_logit;
-    row.slope = -per_logit * 5.2829453113566525e+269;  // 2^896
+    row.wide_max = Row::widen(top);
+    row.slope = per_logit * 5.2829453113566525e+269;  // 2^896
     row.bucket_scale = (float)(inv_t * 64.0);
     const int top_k = p.top_k ? p.top_k[b] : p.top_k_all;
     const double top_p = p.top_p ? (double)p.top_p[b] : p.top_p_all, min_p = p.min_p ? (double)p.min_p[b] : p.min_p_all;

@@ -318,3 +318,67 @@ def test_logits_past_32_bits(dev):
     ids, probs = lb.sample(logits, torch.from_numpy(u).to(dev).repeat(reps), top_p=0.8)
     assert (ids.view(reps, 8) == ids[:8]).all() and (probs.view(reps, 8) == probs[:8]).all()
     check(dev, base, u, p=0.8)
+
+
+FAR_SETTINGS = [dict(), dict(k=1), dict(k=40), dict(p=0.9), dict(mp=0.05), dict(k=40, p=0.9, mp=0.05)]
+
+
+def check_drawn(dev, logits, u, t, s):
+    """As check, and every row with a finite logit gives a token and a probability."""
+    import lloom_b200 as lb
+
+    check(dev, logits, u, t=t, **s)
+    ids, probs = lb.sample(logits.to(dev), torch.from_numpy(np.asarray(u, np.float32)).to(dev), t, s.get("k", 0), s.get("p", 1.0), s.get("mp", 0.0))
+    assert (ids >= 0).all() and (probs > 0).all() and (probs <= 1).all()
+
+
+@pytest.mark.parametrize("v", [300, 20000])
+@pytest.mark.parametrize("t", [1e-6, 1e-9, 1e-12, 1e-14, 1e-15, 1e-16, 1e-17, 1e-18, 1e-20, 1e-22, 1e-24, 1e-26])
+def test_small_temperatures(dev, t, v):
+    """Largest logits with full mantissas over temperatures from 10^-6 to 10^-26: the largest's own weight is 1, and ties of it share the draw."""
+    for x in TYPES.values():
+        logits, u = rand(v, 4, v, x)
+        logits[1, [7, 70, 270]] = logits[1].max()
+        logits[2] = -logits[2].abs() - 3.3
+        logits[3, v // 2:] = logits[3].max()
+        for s in FAR_SETTINGS:
+            check_drawn(dev, logits, u, t, s)
+
+
+@pytest.mark.parametrize("x", ["f32", "bf16"])
+@pytest.mark.parametrize("e", range(50, 92, 3))
+def test_logits_far_from_zero(dev, e, x):
+    """Largest logits around 2^50 to 2^90 at ordinary temperatures, of either sign, alone, tied, and rows of one finite mask value."""
+    v = 3000
+    base, u = rand(e, 5, v)
+    logits = base * 2.0 ** (e - 3)
+    logits[1, [7, 70, 700]] = logits[1].max()
+    logits[2] = -logits[2].abs() - 1.234567 * 2.0 ** e
+    logits[3] = -1.234567 * 2.0 ** e
+    logits[4] = 1.234567 * 2.0 ** e
+    for t in (0.7, 0.8, 1.0):
+        for s in FAR_SETTINGS:
+            check_drawn(dev, logits.to(TYPES[x]), u, t, s)
+
+
+@pytest.mark.parametrize("value", [-1e16, -1e18, -1e20, 1e18, 1e20])
+def test_rows_of_one_far_value(dev, value):
+    logits, u = torch.full((3, 4000), value), np.array([0.0, 0.4, LAST])
+    for t in (0.7, 1.0):
+        for s in FAR_SETTINGS:
+            check_drawn(dev, logits, u, t, s)
+            check_drawn(dev, logits.bfloat16(), u, t, s)
+
+
+@pytest.mark.parametrize("top,t", [(20.0, 3e-7), (100.0, 1e-6), (1000.0, 1e-5), (3e7, 0.9), (1e12, 3e4), (1e-30, 1e-31)])
+def test_close_logits_far_from_zero(dev, top, t):
+    """Logits within some temperatures of the largest, which is 10^7 temperatures and more from zero: weights as exact as near zero."""
+    v = 6000
+    g = torch.Generator().manual_seed(9)
+    ulp = float(np.spacing(np.float32(top)))
+    steps = torch.randint(0, max(2, int(25 * t / ulp)), (4, v), generator=g).double()
+    logits = (top - steps * ulp).float()
+    u = np.array([0.05, 0.31, 0.62, 0.97])
+    for s in (dict(), dict(k=100), dict(k=3000), dict(p=0.9), dict(p=0.5, mp=0.01)):
+        check_drawn(dev, logits, u, t, s)
+        check_drawn(dev, -logits, u, t, s)

@@ -512,6 +512,12 @@ def quantize_weights_host(src, dtype: GgmlDType, nthreads: int = 0, imatrix=None
 def quantize_act(w_dtype: GgmlDType, x: torch.Tensor) -> torch.Tensor:
     """Activation quantizer alone: f32 [m,k] -> canonical Q8_0 / Q8_K blocks, uint8 [m, row_bytes]."""
     L = _lib.lib()
+    if x.dtype != torch.float32:  # the kernel reads four bytes an element
+        raise LloomError(_lib.ERR_DTYPE, "quantize_act", f"values are f32, not {x.dtype}")
+    if not x.is_cuda:
+        raise LloomError(_lib.ERR_DEVICE, "quantize_act", f"input on {x.device}, wanted on a GPU")
+    if x.dim() != 2:
+        raise LloomError(_lib.ERR_SHAPE, "quantize_act", f"input tensor {tuple(x.shape)} is not [m, k]")
     x = x.contiguous()
     m, k = x.shape
     rb = int(L.lloom_b200_act_row_bytes(int(w_dtype), k))

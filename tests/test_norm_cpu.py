@@ -89,3 +89,16 @@ def test_stream_in_place_needs_rows_that_follow_each_other(cuda_lib):
 
     p = 1 << 20
     assert _lib.lib().lloom_b200_rms_norm(p, p + 65536, p, 0, 0, 1e-5, 4, 64, 64, 80, p + 65536, p + 131072, 0, None) == _lib.ERR_SHAPE
+
+
+def test_blocks_of_values_refuse(cuda_lib):
+    """The quantizer reads f32: of anything else it would read past the end."""
+    from lloom_b200 import GgmlDType, LloomError, QActs, _lib
+    from lloom_b200.quantized import quantize_act
+
+    for x, want in ((torch.zeros(2, 256, dtype=torch.float16), _lib.ERR_DTYPE), (torch.zeros(2, 256, dtype=torch.bfloat16), _lib.ERR_DTYPE),
+                    (torch.zeros(2, 256, dtype=torch.int8), _lib.ERR_DTYPE), (torch.zeros(2, 256), _lib.ERR_DEVICE)):
+        for fn in (lambda: QActs.quantize(x, GgmlDType.Q4K), lambda: quantize_act(GgmlDType.Q8_0, x)):
+            with pytest.raises(LloomError) as e:
+                fn()
+            assert e.value.status == want, x.dtype

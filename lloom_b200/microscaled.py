@@ -87,6 +87,8 @@ class MxMatMul:
     """``forward(xs) = xs @ W^T`` over an ``MxTensor``, the activations quantized to the same format on the way."""
 
     def __init__(self, tensor: MxTensor):
+        if not isinstance(tensor, MxTensor):
+            raise LloomError(_lib.ERR_DTYPE, "MxMatMul", f"{type(tensor).__name__} is not an MxTensor")
         self.tensor = tensor
 
     @classmethod

@@ -395,6 +395,8 @@ class QMatMul:
     """``QMatMul::QTensor`` arm (mod.rs:1698-1752): ``forward(xs) = xs @ W^T`` over packed weights."""
 
     def __init__(self, qtensor: QTensor):
+        if not isinstance(qtensor, QTensor):  # a file's MXFP4 tensors are MxTensors
+            raise LloomError(_lib.ERR_DTYPE, "QMatMul", f"{type(qtensor).__name__} is not a QTensor")
         self.qtensor = qtensor
 
     @classmethod

@@ -67,3 +67,15 @@ def test_gguf_lists_mxfp4():
     c = G.Content.read(io.BytesIO(f.getvalue()))
     assert c.tensor_infos["w"].size_in_bytes() == 34
     assert bytes(c.tensor_infos["w"].read_bytes(io.BytesIO(f.getvalue()), c.tensor_data_offset).numpy()) == data
+
+
+def test_products_take_their_own_tensors(cuda_lib):
+    """A GGUF file's tensors are of two kinds: the product of the other kind refuses one at once, not at its first forward."""
+    from lloom_b200 import GgmlDType, LloomError, MxMatMul, MxTensor, QCudaStorage, QMatMul, QTensor, _lib
+
+    q, mx = QTensor(QCudaStorage.load_quantized("cpu", bytes(144 * 4), GgmlDType.Q4K), (4, 256)), MxTensor(None)
+    assert QMatMul.from_qtensor(q).qtensor is q and MxMatMul.from_tensor(mx).tensor is mx
+    for fn, other in ((QMatMul, mx), (QMatMul.from_qtensor, mx), (QMatMul.from_arc, mx), (MxMatMul, q), (MxMatMul.from_tensor, q)):
+        with pytest.raises(LloomError) as e:
+            fn(other)
+        assert e.value.status == _lib.ERR_DTYPE

@@ -416,6 +416,8 @@ class QMatMul:
         """``acts @ W^T`` for activations that are blocks already (``rms_norm(.., act_for=..)``): no quantizer runs, and the
         result is that of ``forward`` on f32 values that quantize to these blocks, bit for bit.  ``dtype``: of the result."""
         qt = self.qtensor
+        if len(qt.shape) != 2:
+            raise LloomError(_lib.ERR_SHAPE, "forward_quantized", f"weight shape {qt.shape} is not [n, k]")
         n, k = qt.shape
         if acts.dtype is not qt.dtype().act or acts.shape[-1] != k:
             raise LloomError(_lib.ERR_SHAPE, "forward_quantized",
@@ -469,6 +471,8 @@ def forward_group(mats: Sequence["QMatMul"], xs: "torch.Tensor | QActs", stores:
     if not 1 <= len(mats) <= 8:
         raise LloomError(_lib.ERR_SHAPE, "forward_group", "1 to 8 matrices")
     tensors = [mm.qtensor for mm in mats]
+    if any(len(t.shape) != 2 for t in tensors):  # of a stack of experts the first two extents would pass for n and k
+        raise LloomError(_lib.ERR_SHAPE, "forward_group", f"weight shapes {[t.shape for t in tensors]} are not [n, k]")
     k = tensors[0].shape[1]
     blocks = isinstance(xs, QActs)
     if all(t.shape[1] == k for t in tensors) and not (blocks and xs.dtype is not tensors[0].dtype().act):

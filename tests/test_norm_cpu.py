@@ -102,3 +102,16 @@ def test_blocks_of_values_refuse(cuda_lib):
             with pytest.raises(LloomError) as e:
                 fn()
             assert e.value.status == want, x.dtype
+
+
+def test_stacks_of_experts_are_no_matrices(cuda_lib):
+    """[8, 256, 256]: its first two extents look like an [n, k] that fits the input."""
+    from lloom_b200 import GgmlDType, LloomError, QActs, QCudaStorage, QMatMul, QTensor, _lib
+    from lloom_b200.quantized import forward_group
+
+    mm = QMatMul(QTensor(QCudaStorage.load_quantized("cpu", bytes(144 * 8 * 256), GgmlDType.Q4K), (8, 256, 256)))
+    acts = QActs(torch.zeros(2, 292, dtype=torch.uint8), GgmlDType.Q8K)
+    for fn in (lambda: mm.forward_quantized(acts), lambda: forward_group([mm], acts), lambda: forward_group([mm], torch.zeros(2, 256))):
+        with pytest.raises(LloomError) as e:
+            fn()
+        assert e.value.status == _lib.ERR_SHAPE and "[n, k]" in str(e.value)

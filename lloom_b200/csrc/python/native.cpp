@@ -325,6 +325,15 @@ PyObject *Storage_experts(PyObject *o, PyObject *const *args, Py_ssize_t nargs) 
 }
 
 
+// A destination of m rows of n f32 values, `ld` apart
+bool out_ok(const at::Tensor &t, c10::Device dev, int64_t m, int64_t n, int64_t &ld) {
+    if (!t.defined() || t.device() != dev || t.layout() != at::kStrided || t.scalar_type() != at::kFloat || t.dim() < 1 || t.size(-1) != n ||
+        t.numel() != m * n || (n > 1 && t.stride(-1) != 1))
+        return false;
+    ld = m > 1 ? t.stride(-2) : n;
+    return m == 1 || (t.dim() == 2 && ld >= n) || t.is_contiguous();
+}
+
 // group(storages, (n, ..), k, x, stores or None, outs or None, whether x is activation blocks) -> list of f32 [.., n_g]
 PyObject *module_group(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
     HANDLE_TH_ERRORS
@@ -353,6 +362,7 @@ PyObject *module_group(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
         n[g] = PyLong_AsLongLong(PyList_GET_ITEM(args[1], g));
         store[g] = stores ? (int)PyLong_AsLong(PyList_GET_ITEM(stores, g)) : LLOOM_STORE_PLAIN;
         if (PyErr_Occurred()) return nullptr;
+        if (store[g] == LLOOM_STORE_MUL_INTO && !outs) Py_RETURN_NONE;  // nothing to multiply into
         n_max = std::max(n_max, n[g]);
         io.overlap = io.overlap && overlaps(st[g]);
     }
@@ -360,8 +370,12 @@ PyObject *module_group(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
     const bool blocks = args[6] == Py_True;
     if (blocks ? !blocks_ok(st[0], x, k) : !acts_ok(st[0], x, k, x_type) || x_type != LLOOM_F32) Py_RETURN_NONE;
     const c10::Device dev = st[0]->data->device();
-    c10::cuda::CUDAGuard guard(dev);
     const int64_t m = x.numel() / x.size(-1);
+    for (Py_ssize_t g = 0; outs && g < G; ++g) {
+        PyObject *item = PyList_GET_ITEM(outs, g);
+        if (!THPVariable_Check(item) || !out_ok(THPVariable_Unpack(item), dev, m, n[g], ld[g])) Py_RETURN_NONE;
+    }
+    c10::cuda::CUDAGuard guard(dev);
     const int64_t need = lloom_b200_workspace_bytes(st[0]->dtype, m, n_max, k);
     if (need <= 0) Py_RETURN_NONE;
     THPObjectPtr list(PyList_New(G));
@@ -370,11 +384,8 @@ PyObject *module_group(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
         PyObject *item;
         if (outs) {
             item = PyList_GET_ITEM(outs, g);
-            if (!THPVariable_Check(item)) Py_RETURN_NONE;
             Py_INCREF(item);
-            const at::Tensor &t = THPVariable_Unpack(item);
-            y[g] = static_cast<float *>(t.data_ptr());
-            ld[g] = t.dim() >= 2 ? t.stride(-2) : t.numel();
+            y[g] = static_cast<float *>(THPVariable_Unpack(item).data_ptr());
         } else {
             c10::SmallVector<int64_t, 5> sizes(x.sizes().begin(), x.sizes().end());
             sizes.back() = n[g];

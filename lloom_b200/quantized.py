@@ -483,7 +483,15 @@ def forward_group(mats: Sequence["QMatMul"], xs: "torch.Tensor | QActs", stores:
     dt, dev = tensors[0].dtype(), tensors[0].device()
     if any(t.dtype() != dt or t.shape[1] != k or t.device() != dev for t in tensors):
         raise LloomError(_lib.ERR_SHAPE, "forward_group", "matrices of a group share dtype, k and device")
-    raise LloomError(_lib.ERR_SHAPE, "forward_group", f"input {tuple(xs.shape)} {xs.dtype}")
+    if stores is not None and 2 in stores and outs is None:
+        raise LloomError(_lib.ERR_NULL, "forward_group", "the multiply-into store needs the destination buffers")
+    if outs is not None:
+        rows = int(np.prod(xs.shape[:-1]))
+        for t, o in zip(tensors, outs):
+            if not isinstance(o, torch.Tensor) or o.dtype != torch.float32 or o.device != dev or o.numel() != rows * t.shape[0]:
+                raise LloomError(_lib.ERR_SHAPE, "forward_group", f"destinations are f32 on {dev}, [.., n] with contiguous rows: one of "
+                                                                  f"{rows} rows of {t.shape[0]} is wanted")
+    raise LloomError(_lib.ERR_SHAPE, "forward_group", f"input {tuple(xs.shape)} {xs.dtype}, {len(tensors)} matrices of rows of {k}")
 
 
 def quantize_weights_host(src, dtype: GgmlDType, nthreads: int = 0, imatrix=None) -> np.ndarray:

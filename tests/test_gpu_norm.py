@@ -302,3 +302,29 @@ def test_offsets_past_32_bits(dev, act):
     for got, want in ((y, y1), (h, h1)):
         assert torch.equal(got[:64], want) and torch.equal(got[-64:], want)
         assert (got.view(reps, 64, -1)[::97] == want).all()
+
+
+@pytest.mark.parametrize("m", [1, 2, 3])
+def test_group_into_destinations(dev, m):
+    """Destinations of a group: matrices, columns of a wider one, more dimensions, a vector for one row; over values and over blocks."""
+    from lloom_b200 import GgmlDType, QMatMul, QTensor, rms_norm
+    from lloom_b200.quantized import forward_group, quantize_weights_host
+
+    rng = np.random.default_rng(m)
+    mats = []
+    for n in (96, 33):
+        w = quantize_weights_host(rng.standard_normal((n, 512)).astype(np.float32), GgmlDType.Q4K)
+        mats.append(QMatMul.from_qtensor(QTensor.from_data(w, GgmlDType.Q4K, (n, 512), dev)))
+    x, w = torch.randn(m, 512, device=dev), torch.ones(512, device=dev)
+    for y in (rms_norm(x, w), rms_norm(x, w, act_for=GgmlDType.Q4K)):
+        want = forward_group(mats, y)
+        wide = torch.full((m, 200), 7.0, device=dev)
+        kinds = [[torch.empty(m, 96, device=dev), torch.empty(m, 33, device=dev)], [wide[:, 3:99], wide[:, 120:153]],
+                 [torch.empty(1, m, 96, device=dev), torch.empty(m, 1, 33, device=dev)]]
+        if m == 1:
+            kinds.append([torch.empty(96, device=dev), torch.empty(33, device=dev)])
+        for outs in kinds:
+            got = forward_group(mats, y, outs=outs)
+            for a, b, o in zip(want, got, outs):
+                assert b is o and torch.equal(a, b.reshape(a.shape))
+        assert (wide[:, :3] == 7).all() and (wide[:, 99:120] == 7).all() and (wide[:, 153:] == 7).all()

@@ -115,3 +115,20 @@ def test_stacks_of_experts_are_no_matrices(cuda_lib):
         with pytest.raises(LloomError) as e:
             fn()
         assert e.value.status == _lib.ERR_SHAPE and "[n, k]" in str(e.value)
+
+
+def test_group_refuses_destinations_that_do_not_fit(cuda_lib):
+    """Every destination is written as f32 rows of n: another type, device or size would be written past its end."""
+    from lloom_b200 import GgmlDType, LloomError, QActs, QCudaStorage, QMatMul, QTensor, _lib
+    from lloom_b200.quantized import forward_group
+
+    mm = QMatMul(QTensor(QCudaStorage.load_quantized("cpu", bytes(144 * 4), GgmlDType.Q4K), (4, 256)))
+    for x in (torch.zeros(2, 256), QActs(torch.zeros(2, 292, dtype=torch.uint8), GgmlDType.Q8K)):
+        for out in (torch.zeros(2, 4, dtype=torch.float16), torch.zeros(1, 4), torch.zeros(2, 5), torch.zeros(8), torch.zeros(2, 8)[:, ::2], torch.zeros(4, 2).t(),
+                    torch.zeros(1, 4).expand(2, 4), torch.zeros(2, 4, device="meta"), None):
+            with pytest.raises(LloomError) as e:
+                forward_group([mm], x, outs=[out])
+            assert e.value.status == _lib.ERR_SHAPE
+        with pytest.raises(LloomError) as e:
+            forward_group([mm], x, stores=[2])
+        assert e.value.status == _lib.ERR_NULL

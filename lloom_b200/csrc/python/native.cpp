@@ -20,6 +20,7 @@
 #include <c10/cuda/CUDAStream.h>
 
 #include <map>
+#include <memory>
 #include <mutex>
 #include <utility>
 #include <vector>
@@ -41,30 +42,85 @@ PyObject *fail(int status, const char *where) {
     return nullptr;
 }
 
-// Grow-only scratch per (device, stream): launches on different streams never share a buffer.  A buffer that has been
-// outgrown stays alive: a CUDA graph captured earlier may hold its address.  A call that is being captured gets memory of its own, which its graph
-// keeps: graphs captured on one stream may be replayed side by side on others.
+// Grow-only scratch per (device, stream): launches on different streams never share a buffer.  A buffer that has been outgrown stays alive: kernels
+// in flight may still use it.
+// Calls that are being captured share scratch of their own, per capture and stream, because graphs captured on one stream may be replayed side by
+// side on others.  The graph holds it by a user object, and so does everything instantiated from the graph, whoever captures: outside of torch's own
+// captures the allocator would give the memory to others as soon as the call has returned.
 struct Workspaces {
+    struct Captured {
+        std::pair<unsigned long long, cudaStream_t> key;
+        at::Tensor buf;
+        std::vector<at::Tensor> outgrown;
+    };
     std::mutex mu;
     std::map<std::pair<int, cudaStream_t>, at::Tensor> bufs;
     std::vector<at::Tensor> retired;
+    std::map<std::pair<unsigned long long, cudaStream_t>, Captured *> captured;
+    std::mutex released_mu;
+    std::vector<Captured *> released;  // of graphs that are gone; freed by the next call
 
-    at::Tensor get(c10::Device dev, cudaStream_t stream, int64_t bytes) {
-        cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
-        if (cudaStreamIsCapturing(stream, &capture) == cudaSuccess && capture != cudaStreamCaptureStatusNone)
-            return at::detail::empty_cuda({std::max<int64_t>(bytes, 512)}, at::kByte, dev, std::nullopt);
-        std::lock_guard<std::mutex> lock(mu);
-        at::Tensor &buf = bufs[{dev.index(), stream}];
-        if (!buf.defined() || buf.numel() < bytes) {
-            if (buf.defined()) retired.push_back(buf);
-            buf = at::detail::empty_cuda({std::max<int64_t>(bytes, 1 << 20)}, at::kByte, dev, std::nullopt);
+    at::Tensor get(c10::Device dev, cudaStream_t stream, int64_t bytes);
+    at::Tensor get_captured(c10::Device dev, cudaStream_t stream, int64_t bytes);
+    void drop_released() {
+        std::vector<Captured *> gone;
+        {
+            std::lock_guard<std::mutex> lock(released_mu);
+            gone.swap(released);
         }
-        return buf;
+        for (Captured *c : gone) {
+            captured.erase(c->key);
+            delete c;
+        }
     }
 };
 Workspaces &workspaces() {
     static Workspaces *w = new Workspaces;  // never destroyed: the CUDA context may be gone by then
     return *w;
+}
+
+// The last graph that holds this scratch is gone.  A thread of the driver may call this: no CUDA call, no lock that is held over one.
+void release_captured(void *p) {
+    std::lock_guard<std::mutex> lock(workspaces().released_mu);
+    workspaces().released.push_back(static_cast<Workspaces::Captured *>(p));
+}
+
+at::Tensor Workspaces::get_captured(c10::Device dev, cudaStream_t stream, int64_t bytes) {
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    cudaGraph_t graph = nullptr;
+    C10_CUDA_CHECK(cudaStreamGetCaptureInfo(stream, &status, &id, &graph));
+    Captured *&c = captured[{id, stream}];
+    if (!c) {
+        auto fresh = std::make_unique<Captured>();
+        fresh->key = {id, stream};
+        cudaUserObject_t object;
+        C10_CUDA_CHECK(cudaUserObjectCreate(&object, fresh.get(), release_captured, 1, cudaUserObjectNoDestructorSync));
+        c = fresh.release();  // the object's now
+        const cudaError_t e = cudaGraphRetainUserObject(graph, object, 1, cudaGraphUserObjectMove);
+        if (e != cudaSuccess) cudaUserObjectRelease(object, 1);
+        C10_CUDA_CHECK(e);
+    }
+    if (!c->buf.defined() || c->buf.numel() < bytes) {
+        at::Tensor larger = at::detail::empty_cuda({std::max<int64_t>(bytes, 1 << 16)}, at::kByte, dev, std::nullopt);
+        if (c->buf.defined()) c->outgrown.push_back(c->buf);
+        c->buf = larger;
+    }
+    return c->buf;
+}
+
+at::Tensor Workspaces::get(c10::Device dev, cudaStream_t stream, int64_t bytes) {
+    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+    const bool capturing = cudaStreamIsCapturing(stream, &capture) == cudaSuccess && capture == cudaStreamCaptureStatusActive;
+    std::lock_guard<std::mutex> lock(mu);
+    drop_released();
+    if (capturing) return get_captured(dev, stream, bytes);
+    at::Tensor &buf = bufs[{dev.index(), stream}];
+    if (!buf.defined() || buf.numel() < bytes) {
+        if (buf.defined()) retired.push_back(buf);
+        buf = at::detail::empty_cuda({std::max<int64_t>(bytes, 1 << 20)}, at::kByte, dev, std::nullopt);
+    }
+    return buf;
 }
 
 struct Storage {

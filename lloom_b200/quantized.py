@@ -75,8 +75,8 @@ def _native():
 class _Workspace:
     """Grow-only scratch per (device, stream), the role of fast_mmvq.rs:44-81 / fast_mmq.rs:135-174.
 
-    Launches on different streams never share a buffer.  A buffer that has been outgrown is kept alive for the
-    life of the process instead of being freed: a CUDA graph captured earlier may still hold its address."""
+    Launches on different streams never share a buffer, nor do calls that are being captured with any outside of
+    their graph: theirs lives as long as the graph and what was instantiated from it, whoever captures."""
 
     @classmethod
     def get(cls, device: torch.device, nbytes: int) -> torch.Tensor:

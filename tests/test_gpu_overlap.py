@@ -83,3 +83,69 @@ def test_switch_decides_for_every_storage(dev, oracle, dt, m, k):
                     assert torch.equal(mm.forward(xt), want)
     finally:
         _lib.lib().lloom_b200_set_launch_overlap(start)
+
+
+def _scratch_users(dev):
+    """Forwards that need scratch: a quantized product and a microscaled one of more rows than their prologues quantize."""
+    import lloom_b200 as lb
+    from lloom_b200.quantized import quantize_weights_host
+
+    n, k, m = 512, 1024, 40
+    rng = np.random.default_rng(3)
+    w = rng.standard_normal((n, k)).astype(np.float32)
+    q = lb.QMatMul.from_qtensor(lb.QTensor.from_data(quantize_weights_host(w, 12), 12, (n, k), dev))
+    mx = lb.MxMatMul.from_tensor(lb.MxTensor.quantize(torch.from_numpy(w).to(dev)))
+    x = torch.randn(m, k, device=dev)
+    return lambda: (q.forward(x), mx.forward(x)), x
+
+
+def test_scratch_of_graphs_that_torch_does_not_capture():
+    """A capture by the runtime's own calls has no pool of memory: what the allocator gives away behind it is not written by replays."""
+    rt = pytest.importorskip("cuda.bindings.runtime")
+    dev = torch.device("cuda:0")
+    step, x = _scratch_users(dev)
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        want = step()  # first forwards wait for their weights
+        s.synchronize()
+        err, = rt.cudaStreamBeginCapture(s.cuda_stream, rt.cudaStreamCaptureMode.cudaStreamCaptureModeRelaxed)
+        assert int(err) == 0
+        got = step()
+        err, graph = rt.cudaStreamEndCapture(s.cuda_stream)
+        assert int(err) == 0
+        err, run = rt.cudaGraphInstantiate(graph, 0)
+        assert int(err) == 0
+        others = [torch.full((size,), 0x5a, dtype=torch.uint8, device=dev) for size in [1 << b for b in range(9, 23)] * 4]
+        x.copy_(torch.randn_like(x))
+        want = step()
+        for _ in range(2):
+            err, = rt.cudaGraphLaunch(run, s.cuda_stream)
+            assert int(err) == 0
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert all((t == 0x5a).all() for t in others)
+    assert int(rt.cudaGraphExecDestroy(run)[0]) == 0 and int(rt.cudaGraphDestroy(graph)[0]) == 0
+
+
+def test_scratch_goes_with_its_graph():
+    """Graphs one after another hold no more memory than one of them does."""
+    import gc
+    import time
+
+    dev = torch.device("cuda:0")
+    step, _ = _scratch_users(dev)
+    step()
+    held = []
+    for _ in range(12):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = step()
+        g.replay()
+        torch.cuda.synchronize()
+        del g, out
+        gc.collect()
+        time.sleep(0.05)  # the driver drops what a graph held on a thread of its own
+        step()
+        torch.cuda.synchronize()
+        held.append(torch.cuda.memory_allocated())
+    assert held[-1] <= held[1], held

@@ -574,6 +574,10 @@ PyObject *MxStorage_dequantize(PyObject *o, PyObject *f16) {
     END_HANDLE_TH_ERRORS
 }
 
+// As for Storage, but the first forward always waits: the kernel in front may be the one that writes the image, which is this package's own
+bool overlaps(const MxStorage *self) { return lloom::launch_overlap() != 0 && self->settled; }
+PyObject *MxStorage_overlaps(PyObject *o, PyObject *) { return PyBool_FromLong(overlaps(reinterpret_cast<MxStorage *>(o))); }
+
 // forward(x [.., k]) -> [.., n] of x's type
 PyObject *MxStorage_forward(PyObject *o, PyObject *const *args, Py_ssize_t nargs) {
     HANDLE_TH_ERRORS
@@ -594,9 +598,8 @@ PyObject *MxStorage_forward(PyObject *o, PyObject *const *args, Py_ssize_t nargs
     at::Tensor y = at::detail::empty_cuda(sizes, x.scalar_type(), dev, std::nullopt);
     const cudaStream_t stream = stream_of(dev);
     const at::Tensor ws = workspaces().get(dev, stream, need);
-    const int mode = lloom::launch_overlap();
     const int rc = lloom::mx_forward(self->image->const_data_ptr(), x.const_data_ptr(), x_type, y.data_ptr(), x_type, m, self->n, self->k,
-                                     self->n, ws.data_ptr(), ws.numel(), stream, mode > 0 || (mode < 0 && self->settled));
+                                     self->n, ws.data_ptr(), ws.numel(), stream, overlaps(self));
     if (rc != LLOOM_OK) return fail(rc, "mx_fwd");
     self->settled = true;
     return THPVariable_Wrap(y);
@@ -759,6 +762,7 @@ PyMethodDef mx_methods[] = {{"forward", FAST(MxStorage_forward), METH_FASTCALL, 
                             {"to_blocks", MxStorage_to_blocks, METH_NOARGS, nullptr},
                             {"shape", MxStorage_shape, METH_NOARGS, nullptr},
                             {"device", MxStorage_device, METH_NOARGS, nullptr},
+                            {"overlaps", MxStorage_overlaps, METH_NOARGS, nullptr},
                             {nullptr, nullptr, 0, nullptr}};
 
 PyMethodDef module_methods[] = {{"group", FAST(module_group), METH_FASTCALL, nullptr},

@@ -149,3 +149,25 @@ def test_scratch_goes_with_its_graph():
         torch.cuda.synchronize()
         held.append(torch.cuda.memory_allocated())
     assert held[-1] <= held[1], held
+
+
+@pytest.mark.parametrize("m", [1, 40, 200])
+def test_first_microscaled_forward_waits(m):
+    """Whatever the switch says: the kernel in front may be the one that writes the image."""
+    import lloom_b200 as lb
+    from lloom_b200 import _lib
+
+    dev, switch = torch.device("cuda:0"), _lib.lib().lloom_b200_set_launch_overlap
+    w, x = torch.randn(384, 1024, device=dev), torch.randn(m, 1024, device=dev)
+    start = switch(-1)
+    try:
+        want = lb.MxMatMul(lb.MxTensor.quantize(w)).forward(x)
+        for mode, early in ((1, True), (-1, True), (0, False)):
+            switch(mode)
+            t = lb.MxTensor.quantize(w)
+            assert not t._native.overlaps()
+            for _ in range(3):
+                assert torch.equal(lb.MxMatMul(t).forward(x), want)
+                assert t._native.overlaps() == early
+    finally:
+        switch(start)

@@ -16,6 +16,7 @@
 #include <torch/extension.h>
 
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
@@ -470,6 +471,7 @@ struct MxStorage {
     at::Tensor *image;
     int64_t n, k;
     bool settled;
+    cudaStream_t home, last;  // where the image was allocated, and the stream of its last use
 };
 PyTypeObject MxStorageType = {PyVarObject_HEAD_INIT(nullptr, 0)};
 
@@ -477,6 +479,8 @@ void MxStorage_dealloc(PyObject *o) {
     delete reinterpret_cast<MxStorage *>(o)->image;
     Py_TYPE(o)->tp_free(o);
 }
+
+cudaStream_t stream_of(c10::Device dev) { return c10::cuda::getCurrentCUDAStream(dev.index()).stream(); }
 
 // An image of its own for [n, k], not yet written; null with an exception
 MxStorage *mx_new(int64_t n, int64_t k, c10::Device dev) {
@@ -486,6 +490,7 @@ MxStorage *mx_new(int64_t n, int64_t k, c10::Device dev) {
     st->n = n;
     st->k = k;
     st->settled = false;
+    st->home = st->last = stream_of(dev);
     try {
         st->image = new at::Tensor(at::detail::empty_cuda({lloom_b200_mx_image_bytes(n, k)}, at::kByte, dev, std::nullopt));
     } catch (...) {
@@ -495,7 +500,14 @@ MxStorage *mx_new(int64_t n, int64_t k, c10::Device dev) {
     return st;
 }
 
-cudaStream_t stream_of(c10::Device dev) { return c10::cuda::getCurrentCUDAStream(dev.index()).stream(); }
+// The current stream, which is about to read the image.  Nobody but this storage holds that, so it tells the allocator of streams other than the
+// image's own: the memory may go to others only when they have finished with it.
+cudaStream_t stream_to_read(MxStorage *self) {
+    const c10::cuda::CUDAStream stream = c10::cuda::getCurrentCUDAStream(self->image->device().index());
+    if (stream.stream() != self->home && stream.stream() != self->last) c10::cuda::CUDACachingAllocator::recordStream(self->image->storage().data_ptr(), stream);
+    self->last = stream.stream();
+    return stream.stream();
+}
 
 // mx_quantize(x [.., k]) -> storage of [rows, k]
 PyObject *module_mx_quantize(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
@@ -554,7 +566,7 @@ PyObject *MxStorage_to_blocks(PyObject *o, PyObject *) {
     const c10::Device dev = self->image->device();
     c10::cuda::CUDAGuard guard(dev);
     at::Tensor out = at::detail::empty_cuda({self->n, self->k / 32 * 17}, at::kByte, dev, std::nullopt);
-    const int rc = lloom_b200_mx_to_blocks(self->image->const_data_ptr(), self->n, self->k, out.data_ptr(), stream_of(dev));
+    const int rc = lloom_b200_mx_to_blocks(self->image->const_data_ptr(), self->n, self->k, out.data_ptr(), stream_to_read(self));
     if (rc != LLOOM_OK) return fail(rc, "mx_to_blocks");
     return THPVariable_Wrap(out);
     END_HANDLE_TH_ERRORS
@@ -567,7 +579,7 @@ PyObject *MxStorage_dequantize(PyObject *o, PyObject *f16) {
     const c10::Device dev = self->image->device();
     c10::cuda::CUDAGuard guard(dev);
     at::Tensor out = at::detail::empty_cuda({self->n, self->k}, f16 == Py_True ? at::kHalf : at::kFloat, dev, std::nullopt);
-    const int rc = lloom::mx_dequantize(self->image->const_data_ptr(), self->n, self->k, out.data_ptr(), f16 == Py_True, stream_of(dev),
+    const int rc = lloom::mx_dequantize(self->image->const_data_ptr(), self->n, self->k, out.data_ptr(), f16 == Py_True, stream_to_read(self),
                                         lloom::launch_overlap() != 0);
     if (rc != LLOOM_OK) return fail(rc, "mx_dequantize");
     return THPVariable_Wrap(out);
@@ -596,7 +608,7 @@ PyObject *MxStorage_forward(PyObject *o, PyObject *const *args, Py_ssize_t nargs
     c10::SmallVector<int64_t, 5> sizes(x.sizes().begin(), x.sizes().end());
     sizes.back() = self->n;
     at::Tensor y = at::detail::empty_cuda(sizes, x.scalar_type(), dev, std::nullopt);
-    const cudaStream_t stream = stream_of(dev);
+    const cudaStream_t stream = stream_to_read(self);
     const at::Tensor ws = workspaces().get(dev, stream, need);
     const int rc = lloom::mx_forward(self->image->const_data_ptr(), x.const_data_ptr(), x_type, y.data_ptr(), x_type, m, self->n, self->k,
                                      self->n, ws.data_ptr(), ws.numel(), stream, overlaps(self));

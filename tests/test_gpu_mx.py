@@ -350,3 +350,27 @@ def test_offsets_past_32_bits(dev, m, n, k):
         for cols in (slice(0, 100), slice(n - 100, n)):
             assert torch.equal(y[rows, cols], want)
     assert (y.view(m // 40, -1)[:: max(1, m // 400)] == y[:40].reshape(-1)).all()
+
+
+@pytest.mark.parametrize("m", [1, 40])
+def test_tensor_dropped_while_another_stream_reads_it(dev, m):
+    """Its memory goes to others only when that stream has finished with it."""
+    import lloom_b200 as lb
+
+    w, x = torch.randn(1024, 4096, device=dev), torch.randn(m, 4096, device=dev)
+    t = lb.MxTensor.quantize(w)
+    size = t._native.to_blocks().shape[0] // 128 * 16 * (128 * 128 + 1024)
+    want = [lb.MxMatMul(t).forward(x), t.dequantize(), t._native.to_blocks()]
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for use, ref in zip((lambda t: lb.MxMatMul(t).forward(x), lambda t: t.dequantize(), lambda t: t._native.to_blocks()), want):
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(40_000_000)
+            got = use(t)
+        del t
+        others = [torch.full((size,), 0x77, dtype=torch.uint8, device=dev) for _ in range(3)]
+        torch.cuda.synchronize()
+        assert torch.equal(got, ref)
+        del others
+        t = lb.MxTensor.quantize(w)
+        torch.cuda.synchronize()

@@ -16,7 +16,7 @@
 // codes of half of the rows and the scales of all, so that a CTA of the pair copies one piece.
 //
 // Bound by: one row of small matrices, the latency of one launch and a chain of copy, products, reduction ([1024, 4096] 4.3 us); a few rows of large
-// ones, reading the weights (8 x [14336, 4096] 7.2 us, 31 MB: 4.3 TB/s with all of start and end); many rows, the tensor cores and
+// ones, reading the weights (8 x [14336, 4096] 7.4 us, 31 MB: 4.2 TB/s with all of start and end); many rows, the tensor cores and
 // what L2 gives an SM (2048 x [14336, 4096] 51 us, 4.7 PFLOP/s, the tensor pipe 75 % busy; 73 with the quantizer and from new inputs; 512 x [4096, 14336]
 // 26 us: 2.3).  Quantizing 512 x 4096 bf16 takes
 // 2.4 us, reading the values back as f32 4.3.
@@ -818,7 +818,7 @@ MxTiles mx_pair_tiles(int64_t m, int64_t n, int pairs) {
 //   pairs of CTAs past 128 rows, if K is short or they have tiles for half of the SMs: their own K is not split.  Split / pairs:
 //     [1024, 4096] 128 rows 9.2 / 10.4, 192 10.8 / 10.5, 256 12.5 / 10.8; [4096, 4096] 128 10.9 / 10.8, 192 12.6 / 11.1;
 //     [14336, 4096] 96 11.6 / 12.3, 128 12.8 / 12.2, 256 17.7 / 16.5; [4096, 14336] 128 15.8 / 22.2, 384 22.7 / 25.0; [8192, 8192] 384 21.5 / 19.8
-//   split: K over as many CTAs of a cluster as there are SMs for, two units at least to each.
+//   split: K over as many CTAs of a cluster, up to eight, as there are SMs for, one unit at least to each.
 //   quantize: the quantizer in the product's prologue where a CTA has up to 32 (row, unit of K) pairs to do, four to a warp: beyond, all CTAs
 //     repeating the work costs more than a launch.  In the prologue / in a launch of its own: 1 x [1024, 4096] 4.5 / 5.9, 16 x [1024, 4096] (32) 5.9 / 6.3,
 //     8 x [4096, 4096] (32) 6.9 / 7.0, 16 x [4096, 4096] (64) 8.8 / 7.2, 1 x [14336, 4096] (16) 6.7 / 7.7, 4 x [14336, 4096] (64) 9.3 / 8.0

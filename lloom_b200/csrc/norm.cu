@@ -5,8 +5,9 @@
 //   inv = f32(1 / sqrt(sum(h * h) / k + eps))     the sum and everything up to inv in 64 bits
 //   y = f32(f32(h * inv) * w)                     stored as T, or as Q8_0 / Q8_K blocks of these f32 values
 //
-// Squares of f32 values are exact in 64 bits and their sum is off by 1e-16, so that inv, and with it every code of the 8-bit
-// blocks, is a function of the inputs and not of how the row was split over threads.
+// Squares of f32 values are exact in 64 bits and their sum is off by 1e-16.  How a row is split over threads (which depends on the batch and on
+// alignment) changes the last bits of the sum in one row of three, and inv, and with it codes of the 8-bit blocks, only where 1 / sqrt lies within a few
+// units of 2^-53 of the middle between two f32 values: about one row in 10^8.
 //
 // Bound by memory (x and r read once, h and y written once: the row stays in registers between the sum and the output) or,
 // for a few rows, by the latency of one launch, two loads and a reduction over the row.
@@ -355,8 +356,9 @@ int rms_norm(const void *x, const void *residual, const void *weight, int x_type
     const bool wide = blocks ? phase(x) == 0 && ldx * es % 16 == 0 && (!residual || (phase(residual) == 0 && phase(h) == 0 && ldr * es % 16 == 0))
                              : steps && phase(y) == phase(x) && (!residual || (phase(residual) == phase(x) && phase(h) == phase(x)));
     // Threads: a piece each and a row per CTA, so that a row alone waits for memory once.  Many rows of halves: two pieces each, in 40 registers, so
-    // that six rows of 4096 are in flight on an SM instead of four (2048 x 4096 bf16: 12.0 us, one piece each 15.8; 592 rows: level).  (With
-    // f32 four rows in flight are enough: 22.6 us are 5.9 TB/s.)  Rows of up to 32 pieces share a CTA of 256 threads.
+    // that six rows of 4096 are in flight on an SM instead of four.  us of a call in a captured chain with changing inputs, two pieces / one, bf16 with a
+    // residual: 2048 x 4096 13.0 / 16.0, 1024 x 4096 8.3 / 9.4, 592 x 4096 6.7 / 6.1, 2048 x 2048 7.9 / 8.5, 2048 x 8192 24.5 / 37.9.  (With
+    // f32 four rows in flight are enough: 22.7 us are 5.9 TB/s.)  Rows of up to 32 pieces share a CTA of 256 threads.
     const int pieces = !wide ? kAnywhere : phase(x) == 0 && phase(weight) == 0 && k % 8 == 0 && ldx * es % 16 == 0 ? kWhole : kEdges;
     const int64_t octets = (k + 7) / 8 + (pieces == kEdges ? 1 : 0);
     const bool pairs = x_type != LLOOM_F32 && m >= 592 && octets > 64 && octets <= 1024;

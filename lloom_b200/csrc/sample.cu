@@ -17,9 +17,9 @@
 // degree 9; relative error below 3e-14 at every temperature and size of the logits.
 //
 // Bound by latency for a few rows: a launch, one read of DRAM, six to eight cluster barriers of about a microsecond with short passes between
-// them (1 x 128256 f32 with all filters 15.3 us, 7 x 50257 bf16 with top-p 33).  For many rows by instruction issue and barriers
+// them (1 x 128256 f32 with all filters 15.4 us, 7 x 50257 bf16 with top-p 33).  For many rows by instruction issue and barriers
 // (issue slots 54 % taken, the 64-bit pipe 10 %, shared memory's 25 %; half of the instructions are per logit, half per CTA): 64 x 128256 f32, 33 MB,
-// settings of their own, 68 us.
+// settings of their own, 70 us.
 // There a row read from L2 in every pass by fewer CTAs, all rows at once, was faster for alike rows (75 us for 85) and slower for unlike ones (126 for 84).
 #include <mutex>
 #include <type_traits>

@@ -16,8 +16,9 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, residual:
     Returns ``y``, or ``(y, h)`` where a residual is given.  ``y`` has x's type; with ``act_for``, the dtype of the weights that
     read it next, it is a ``QActs`` of their block type instead, for ``QMatMul.forward_quantized`` and ``forward_group``.
     ``x`` and ``residual`` are f32, f16 or bf16, of one type and shape, contiguous or matrices with contiguous rows; ``weight``
-    has any of the three types.  The blocks are those of the f32 values of ``y``, whose every rounding is defined, so they do
-    not depend on how a row is summed."""
+    has any of the three types.  The blocks are those of the f32 values of ``y``, whose every rounding is defined but the last bits
+    of a 64-bit sum: a row has the same blocks in every batch, but for about one in 10^8, whose 1 / sqrt lies on the border of two
+    f32 values."""
     act = None if act_for is None else act_type(act_for)
     got = _native().rms_norm(x, weight, eps, residual, -1 if act is None else act)
     if got is None:

@@ -387,8 +387,8 @@ bool out_ok(const at::Tensor &t, c10::Device dev, int64_t m, int64_t n, int64_t 
     if (!t.defined() || t.device() != dev || t.layout() != at::kStrided || t.scalar_type() != at::kFloat || t.dim() < 1 || t.size(-1) != n ||
         t.numel() != m * n || (n > 1 && t.stride(-1) != 1))
         return false;
-    ld = m > 1 ? t.stride(-2) : n;
-    return m == 1 || (t.dim() == 2 && ld >= n) || t.is_contiguous();
+    ld = t.dim() == 2 && m > 1 ? t.stride(0) : n;  // (the stride of an extent of 1 says nothing)
+    return m == 1 || (t.dim() == 2 ? ld >= n : t.is_contiguous());
 }
 
 // group(storages, (n, ..), k, x, stores or None, outs or None, whether x is activation blocks) -> list of f32 [.., n_g]

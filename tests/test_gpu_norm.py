@@ -328,3 +328,19 @@ def test_group_into_destinations(dev, m):
             for a, b, o in zip(want, got, outs):
                 assert b is o and torch.equal(a, b.reshape(a.shape))
         assert (wide[:, :3] == 7).all() and (wide[:, 99:120] == 7).all() and (wide[:, 153:] == 7).all()
+
+
+def test_group_into_destinations_of_odd_strides(dev):
+    """An extent of 1 may have any stride: it does not say how far rows are apart."""
+    from lloom_b200 import GgmlDType, QMatMul, QTensor
+    from lloom_b200.quantized import forward_group, quantize_weights_host
+
+    w = quantize_weights_host(np.random.default_rng(0).standard_normal((64, 512)).astype(np.float32), GgmlDType.Q4K)
+    mm = QMatMul.from_qtensor(QTensor.from_data(w, GgmlDType.Q4K, (64, 512), dev))
+    x, buf = torch.randn(3, 512, device=dev), torch.zeros(1000, device=dev)
+    want = forward_group([mm], x)[0]
+    out = buf.as_strided((3, 1, 64), (64, 200, 1))
+    assert out.is_contiguous()
+    assert torch.equal(forward_group([mm], x, outs=[out])[0].view(3, 64), want) and not buf[192:].any()
+    one = buf.as_strided((1, 64), (1, 1), 400)
+    assert torch.equal(forward_group([mm], x[:1], outs=[one])[0], forward_group([mm], x[:1])[0]) and not buf[464:].any()

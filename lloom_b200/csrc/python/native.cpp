@@ -45,9 +45,10 @@ PyObject *fail(int status, const char *where) {
 
 // Grow-only scratch per (device, stream): launches on different streams never share a buffer.  A buffer that has been outgrown stays alive: kernels
 // in flight may still use it.
-// Calls that are being captured share scratch of their own, per capture and stream, because graphs captured on one stream may be replayed side by
-// side on others.  The graph holds it by a user object, and so does everything instantiated from the graph, whoever captures: outside of torch's own
-// captures the allocator would give the memory to others as soon as the call has returned.
+// A call that is being captured gets scratch of its own, because graphs captured on one stream may be replayed side by side on others.  In torch's
+// captures it comes from the graph's pool, and stays there.  In a capture by the runtime's own calls the allocator would give it to others as soon as
+// the call has returned: there it is kept, per capture and stream, and a user object ties it to the graph and all that is instantiated from it.  (Not
+// in torch's captures too: a replay of a graph with a user object takes 2.6 us longer.)
 struct Workspaces {
     struct Captured {
         std::pair<unsigned long long, cudaStream_t> key;
@@ -58,11 +59,13 @@ struct Workspaces {
     std::map<std::pair<int, cudaStream_t>, at::Tensor> bufs;
     std::vector<at::Tensor> retired;
     std::map<std::pair<unsigned long long, cudaStream_t>, Captured *> captured;
+    unsigned long long last_pooled = ~0ull;  // capture, by torch
     std::mutex released_mu;
     std::vector<Captured *> released;  // of graphs that are gone; freed by the next call
 
     at::Tensor get(c10::Device dev, cudaStream_t stream, int64_t bytes);
     at::Tensor get_captured(c10::Device dev, cudaStream_t stream, int64_t bytes);
+    bool pooled(unsigned long long capture, const at::Tensor &t);
     void drop_released() {
         std::vector<Captured *> gone;
         {
@@ -86,28 +89,45 @@ void release_captured(void *p) {
     workspaces().released.push_back(static_cast<Workspaces::Captured *>(p));
 }
 
+// Whether what the allocator gives to this capture belongs to its graph: a pool of torch's, or an allocator whose memory is part of the graph.  The
+// allocator's list of segments is all that says so, which is why a capture asks once.
+bool Workspaces::pooled(unsigned long long capture, const at::Tensor &t) {
+    namespace alloc = c10::cuda::CUDACachingAllocator;
+    if (capture == last_pooled) return true;
+    bool yes = alloc::name() != "native";
+    if (!yes) {
+        const size_t at = reinterpret_cast<size_t>(t.const_data_ptr());
+        for (const auto &seg : alloc::snapshot({0, 0}, false).segments)
+            if (seg.device == t.device().index() && at - static_cast<size_t>(seg.address) < static_cast<size_t>(seg.total_size))
+                yes = seg.owner_private_pool_id != c10::MempoolId_t{0, 0};
+    }
+    if (yes) last_pooled = capture;
+    return yes;
+}
+
 at::Tensor Workspaces::get_captured(c10::Device dev, cudaStream_t stream, int64_t bytes) {
     cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
     unsigned long long id = 0;
     cudaGraph_t graph = nullptr;
     C10_CUDA_CHECK(cudaStreamGetCaptureInfo(stream, &status, &id, &graph));
-    Captured *&c = captured[{id, stream}];
-    if (!c) {
-        auto fresh = std::make_unique<Captured>();
-        fresh->key = {id, stream};
-        cudaUserObject_t object;
-        C10_CUDA_CHECK(cudaUserObjectCreate(&object, fresh.get(), release_captured, 1, cudaUserObjectNoDestructorSync));
-        c = fresh.release();  // the object's now
-        const cudaError_t e = cudaGraphRetainUserObject(graph, object, 1, cudaGraphUserObjectMove);
-        if (e != cudaSuccess) cudaUserObjectRelease(object, 1);
-        C10_CUDA_CHECK(e);
+    const auto known = captured.find({id, stream});
+    if (known != captured.end() && known->second->buf.numel() >= bytes) return known->second->buf;
+    const at::Tensor fresh = at::detail::empty_cuda({std::max<int64_t>(bytes, 512)}, at::kByte, dev, std::nullopt);
+    if (known != captured.end()) {
+        known->second->outgrown.push_back(known->second->buf);
+        return known->second->buf = fresh;
     }
-    if (!c->buf.defined() || c->buf.numel() < bytes) {
-        at::Tensor larger = at::detail::empty_cuda({std::max<int64_t>(bytes, 1 << 16)}, at::kByte, dev, std::nullopt);
-        if (c->buf.defined()) c->outgrown.push_back(c->buf);
-        c->buf = larger;
-    }
-    return c->buf;
+    if (pooled(id, fresh)) return fresh;
+    Captured *c = new Captured{{id, stream}, fresh, {}};
+    cudaUserObject_t object;
+    cudaError_t e = cudaUserObjectCreate(&object, c, release_captured, 1, cudaUserObjectNoDestructorSync);
+    if (e != cudaSuccess) delete c;
+    C10_CUDA_CHECK(e);
+    captured[c->key] = c;  // the object owns it
+    e = cudaGraphRetainUserObject(graph, object, 1, cudaGraphUserObjectMove);
+    if (e != cudaSuccess) cudaUserObjectRelease(object, 1);
+    C10_CUDA_CHECK(e);
+    return fresh;
 }
 
 at::Tensor Workspaces::get(c10::Device dev, cudaStream_t stream, int64_t bytes) {

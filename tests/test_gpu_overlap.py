@@ -171,3 +171,32 @@ def test_first_microscaled_forward_waits(m):
                 assert t._native.overlaps() == early
     finally:
         switch(start)
+
+
+def test_scratch_goes_with_a_graph_that_torch_does_not_capture():
+    import time
+
+    rt = pytest.importorskip("cuda.bindings.runtime")
+    dev = torch.device("cuda:0")
+    step, _ = _scratch_users(dev)
+    s, held = torch.cuda.Stream(), []
+    with torch.cuda.stream(s):
+        step()
+        for _ in range(12):
+            s.synchronize()
+            assert int(rt.cudaStreamBeginCapture(s.cuda_stream, rt.cudaStreamCaptureMode.cudaStreamCaptureModeRelaxed)[0]) == 0
+            out = step()
+            err, graph = rt.cudaStreamEndCapture(s.cuda_stream)
+            assert int(err) == 0
+            err, run = rt.cudaGraphInstantiate(graph, 0)
+            assert int(err) == 0 and int(rt.cudaGraphDestroy(graph)[0]) == 0
+            assert int(rt.cudaGraphLaunch(run, s.cuda_stream)[0]) == 0
+            s.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(out, step()))
+            assert int(rt.cudaGraphExecDestroy(run)[0]) == 0
+            del out
+            time.sleep(0.05)  # the driver drops what a graph held on a thread of its own
+            step()
+            s.synchronize()
+            held.append(torch.cuda.memory_allocated())
+    assert held[-1] <= held[1], held

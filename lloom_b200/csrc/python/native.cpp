@@ -20,8 +20,8 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
+#include <atomic>
 #include <map>
-#include <memory>
 #include <mutex>
 #include <utility>
 #include <vector>
@@ -62,15 +62,18 @@ struct Workspaces {
     unsigned long long last_pooled = ~0ull;  // capture, by torch
     std::mutex released_mu;
     std::vector<Captured *> released;  // of graphs that are gone; freed by the next call
+    std::atomic<bool> any_released{false};
 
     at::Tensor get(c10::Device dev, cudaStream_t stream, int64_t bytes);
     at::Tensor get_captured(c10::Device dev, cudaStream_t stream, int64_t bytes);
     bool pooled(unsigned long long capture, const at::Tensor &t);
     void drop_released() {
+        if (!any_released.load(std::memory_order_relaxed)) return;
         std::vector<Captured *> gone;
         {
             std::lock_guard<std::mutex> lock(released_mu);
             gone.swap(released);
+            any_released = false;
         }
         for (Captured *c : gone) {
             captured.erase(c->key);
@@ -87,6 +90,7 @@ Workspaces &workspaces() {
 void release_captured(void *p) {
     std::lock_guard<std::mutex> lock(workspaces().released_mu);
     workspaces().released.push_back(static_cast<Workspaces::Captured *>(p));
+    workspaces().any_released = true;
 }
 
 // Whether what the allocator gives to this capture belongs to its graph: a pool of torch's, or an allocator whose memory is part of the graph.  The
@@ -411,22 +415,20 @@ bool out_ok(const at::Tensor &t, c10::Device dev, int64_t m, int64_t n, int64_t 
     return m == 1 || (t.dim() == 2 ? ld >= n : t.is_contiguous());
 }
 
-// group(storages, (n, ..), k, x, stores or None, outs or None, whether x is activation blocks) -> list of f32 [.., n_g]
+// group(storages, [(n, k), ..], x, stores or None, outs or None, whether x is activation blocks) -> list of f32 [.., n_g]
 PyObject *module_group(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
     HANDLE_TH_ERRORS
-    if (nargs != 7 || !PyList_Check(args[0]) || !PyList_Check(args[1]) || !THPVariable_Check(args[3])) Py_RETURN_NONE;
+    if (nargs != 6 || !PyList_Check(args[0]) || !PyList_Check(args[1]) || !THPVariable_Check(args[2])) Py_RETURN_NONE;
     const Py_ssize_t G = PyList_GET_SIZE(args[0]);
     if (G < 1 || G > LLOOM_B200_MAX_GROUP || PyList_GET_SIZE(args[1]) != G) Py_RETURN_NONE;
-    const int64_t k = PyLong_AsLongLong(args[2]);
-    if (PyErr_Occurred()) return nullptr;
-    const at::Tensor &x = THPVariable_Unpack(args[3]);
-    PyObject *stores = args[4] == Py_None ? nullptr : args[4], *outs = args[5] == Py_None ? nullptr : args[5];
+    const at::Tensor &x = THPVariable_Unpack(args[2]);
+    PyObject *stores = args[3] == Py_None ? nullptr : args[3], *outs = args[4] == Py_None ? nullptr : args[4];
     if ((stores && (!PyList_Check(stores) || PyList_GET_SIZE(stores) != G)) || (outs && (!PyList_Check(outs) || PyList_GET_SIZE(outs) != G)))
         Py_RETURN_NONE;
     Storage *st[LLOOM_B200_MAX_GROUP];
     const void *w[LLOOM_B200_MAX_GROUP];
     float *y[LLOOM_B200_MAX_GROUP];
-    int64_t n[LLOOM_B200_MAX_GROUP], ld[LLOOM_B200_MAX_GROUP], n_max = 0;
+    int64_t n[LLOOM_B200_MAX_GROUP], ld[LLOOM_B200_MAX_GROUP], n_max = 0, k = 0;
     int store[LLOOM_B200_MAX_GROUP];
     FwdIo io;
     io.overlap = true;
@@ -436,7 +438,9 @@ PyObject *module_group(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
         st[g] = reinterpret_cast<Storage *>(s);
         if (st[g]->dtype != st[0]->dtype || st[g]->data->device() != st[0]->data->device()) Py_RETURN_NONE;
         w[g] = st[g]->data->const_data_ptr();
-        n[g] = PyLong_AsLongLong(PyList_GET_ITEM(args[1], g));
+        int64_t k_g;  // (of a stack of experts the first two extents would pass for n and k: shape2 refuses one)
+        if (!shape2(PyList_GET_ITEM(args[1], g), n[g], k_g) || (g > 0 && k_g != k)) return none_or_error();
+        k = k_g;
         store[g] = stores ? (int)PyLong_AsLong(PyList_GET_ITEM(stores, g)) : LLOOM_STORE_PLAIN;
         if (PyErr_Occurred()) return nullptr;
         if (store[g] == LLOOM_STORE_MUL_INTO && !outs) Py_RETURN_NONE;  // nothing to multiply into
@@ -444,7 +448,7 @@ PyObject *module_group(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
         io.overlap = io.overlap && overlaps(st[g]);
     }
     int x_type;
-    const bool blocks = args[6] == Py_True;
+    const bool blocks = args[5] == Py_True;
     if (blocks ? !blocks_ok(st[0], x, k) : !acts_ok(st[0], x, k, x_type) || x_type != LLOOM_F32) Py_RETURN_NONE;
     const c10::Device dev = st[0]->data->device();
     const int64_t m = x.numel() / x.size(-1);

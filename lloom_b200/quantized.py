@@ -471,15 +471,15 @@ def forward_group(mats: Sequence["QMatMul"], xs: "torch.Tensor | QActs", stores:
     if not 1 <= len(mats) <= 8:
         raise LloomError(_lib.ERR_SHAPE, "forward_group", "1 to 8 matrices")
     tensors = [mm.qtensor for mm in mats]
-    if any(len(t.shape) != 2 for t in tensors):  # of a stack of experts the first two extents would pass for n and k
-        raise LloomError(_lib.ERR_SHAPE, "forward_group", f"weight shapes {[t.shape for t in tensors]} are not [n, k]")
-    k = tensors[0].shape[1]
     blocks = isinstance(xs, QActs)
-    if all(t.shape[1] == k for t in tensors) and not (blocks and xs.dtype is not tensors[0].dtype().act):
-        got = _native().group([t.storage._native for t in tensors], [t.shape[0] for t in tensors], k, xs.blocks if blocks else xs,
+    if not (blocks and xs.dtype is not tensors[0].dtype().act):
+        got = _native().group([t.storage._native for t in tensors], [t.shape for t in tensors], xs.blocks if blocks else xs,
                               None if stores is None else list(stores), None if outs is None else list(outs), blocks)
         if got is not None:
             return got
+    if any(len(t.shape) != 2 for t in tensors):
+        raise LloomError(_lib.ERR_SHAPE, "forward_group", f"weight shapes {[t.shape for t in tensors]} are not [n, k]")
+    k = tensors[0].shape[1]
     dt, dev = tensors[0].dtype(), tensors[0].device()
     if any(t.dtype() != dt or t.shape[1] != k or t.device() != dev for t in tensors):
         raise LloomError(_lib.ERR_SHAPE, "forward_group", "matrices of a group share dtype, k and device")
